@@ -18,6 +18,9 @@ E_DEVICE_WAIT, E_OUT_OF_RANGE, E_TOO_LARGE, E_ALLOC = -5, -6, -7, -8
 GEMM_NT, GEMM_NN, GEMM_TN = 0, 1, 2
 ACT = {"none": 0, "relu": 1, "leaky": 2, "sigmoid": 3, "tanh": 4, "gelu": 5, "selu": 6, "mish": 7,
        "swish": 8, "softmax": 9}
+ROTARY_LAYOUT = {"half": 0, "interleaved": 1}
+ROTARY_SCALING = {"plain": 0, "linear": 1, "base": 2, "by_parts": 3}
+TOP_MAX = 2048
 PATH_AUTO, PATH_TC, PATH_SIMT, PATH_SKINNY = 0, 1, 2, 3
 PREP_RAW_HI, PREP_LEFT, PREP_TF32_LO = 1, 2, 4
 
@@ -84,6 +87,17 @@ SIGNATURES = {
     "kai_mix_values_backward_value": (_i, [_i, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "kai_softmax_idx_crossentropy": (_i, [_i, _p, _p, _p, _i64, _i64, _p]),
     "kai_softmax_idx_crossentropy_backward_x": (_i, [_i, _p, _p, _p, _p, _i64, _i64, _p]),
+    "kai_rotary": (_i, [_i, _p, _p, _p, _p] + [_i64] * 6 + [_i, _p, _i64, _i64, _p]),
+    "kai_rotary_backward": (_i, [_i, _p, _p, _p, _p] + [_i64] * 6 + [_i, _p, _i64, _i64, _p]),
+    "kai_rotary_frequencies": (_i, [_i, _p, _i64, C.c_double, _i, C.c_double, C.c_double, C.c_double, _i64, _p]),
+    "kai_gated_linear_forward": (_i, [_i] + [_p] * 8 + [_i64] * 3 + [_i, _p, _p]),
+    "kai_gated_linear_backward": (_i, [_i] + [_p] * 11 + [_i64] * 3 + [_i, _p, _i, _i, _p]),
+    "kai_softmax_top_distill": (_i, [_i] + [_p] * 5 + [_i64] * 3 + [_p, _p]),
+    "kai_softmax_top_distill_backward_x": (_i, [_i] + [_p] * 6 + [_i64] * 3 + [_p, _p]),
+    "kai_softmax_top_distill_step": (_i, [_i] + [_p] * 6 + [_i64] * 3 + [_p, _p]),
+    "kai_softmax_policy_loss": (_i, [_i] + [_p] * 8 + [_i64] * 2 + [_p] * 5),
+    "kai_softmax_policy_loss_backward_x": (_i, [_i] + [_p] * 5 + [_i64] * 2 + [_p, _p]),
+    "kai_softmax_policy_loss_step": (_i, [_i] + [_p] * 9 + [_i64] * 2 + [_p] * 5),
     "kai_sum": (_i, [_i, _p, _p, _i64, _p]),
     "kai_sum_backward": (_i, [_i, _p, _p, _i64, _p]),
 }

@@ -1,5 +1,6 @@
 // C ABI of the sm_100a matmul / Linear path: argument checks, device state, dispatch to the
 // kernel families, and the device allocator.  See include/kai_b200.h for the contract.
+#include <math.h>
 #include <string.h>
 
 #include <map>
@@ -48,6 +49,26 @@ int attn_softmax_axis_backward(float*, const float*, int64_t, int64_t, int64_t, 
 int selftest_bounded_wait(DeviceState*, int64_t, cudaStream_t);
 int ew_layernorm(float*, const float*, float*, int64_t, int64_t, const float*, cudaStream_t);
 int ew_layernorm_backward(float*, const float*, const float*, int64_t, int64_t, const float*, cudaStream_t);
+int rotary(DeviceState*, float*, const float*, const double*, const int64_t*, int64_t, int64_t, int64_t, int64_t, int64_t,
+           int64_t, int, const float*, int64_t, int64_t, int, cudaStream_t);
+int rotary_frequencies(double*, int64_t, double, int, double, double, double, int64_t, cudaStream_t);
+int gated_apply(DeviceState*, float*, float*, float*, const float*, const float*, int64_t, int64_t, int, const float*, int,
+                cudaStream_t);
+int gated_apply_backward(DeviceState*, float*, float*, const float*, const float*, const float*, int64_t, int,
+                         const float*, cudaStream_t);
+int loss_distill(DeviceState*, float*, float*, const float*, const int*, const float*, int64_t, int64_t, int64_t,
+                 const float*, cudaStream_t);
+int loss_distill_backward(DeviceState*, float*, const float*, const float*, const float*, const int*, const float*, int64_t,
+                          int64_t, int64_t, const float*, cudaStream_t);
+int loss_distill_step(DeviceState*, float*, float*, const float*, const float*, const int*, const float*, int64_t, int64_t,
+                      int64_t, const float*, cudaStream_t);
+int loss_policy(DeviceState*, float*, float*, float*, const float*, const int*, const float*, const float*, const float*,
+                int64_t, int64_t, const float*, const float*, const float*, const float*, cudaStream_t);
+int loss_policy_backward(DeviceState*, float*, const float*, const float*, const float*, const int*, int64_t, int64_t,
+                         const float*, cudaStream_t);
+int loss_policy_step(DeviceState*, float*, float*, float*, const float*, const float*, const int*, const float*,
+                     const float*, const float*, int64_t, int64_t, const float*, const float*, const float*, const float*,
+                     cudaStream_t);
 int gemm_simt_grouped(int layout, int count, float* const* c, const float* const* a, const float* const* b, int64_t M,
                       int64_t N, int64_t K, int64_t ldc, const Epilogue& ep, cudaStream_t s);
 void profile_enable(bool on);
@@ -327,6 +348,12 @@ int kai_device_status(int device, int* detail) {
         KAI_CUDA(cudaMemset(st->flag_dev + 1, 0, sizeof(int)));
         return fail(KAI_E_OUT_OF_RANGE, "softmax_idx_crossentropy (replayed): label outside [0, ncol)");
     }
+    // labels of the row losses (their calls never wait for the device)
+    KAI_CUDA(cudaMemcpy(&bad, st->flag_dev + 2, sizeof(int), cudaMemcpyDeviceToHost));
+    if (bad) {
+        KAI_CUDA(cudaMemset(st->flag_dev + 2, 0, sizeof(int)));
+        return fail(KAI_E_OUT_OF_RANGE, "softmax_top_distill / softmax_policy_loss: label outside [0, ncol)");
+    }
     return KAI_OK;
 }
 
@@ -340,7 +367,7 @@ int kai_device_status_clear(int device) {
     st->status_host[1] = 0;
     int stat[2];
     static_status_peek(device, stat, true);
-    KAI_CUDA(cudaMemset(st->flag_dev + 1, 0, sizeof(int)));
+    KAI_CUDA(cudaMemset(st->flag_dev + 1, 0, 2 * sizeof(int)));
     return KAI_OK;
 }
 
@@ -1333,6 +1360,257 @@ int kai_sum_backward(int device, float* pgx, const float* pgy, int64_t nrow, voi
     if (nrow == 0) return KAI_OK;
     if (!pgx) return fail(KAI_E_INVALID_ARG, "sum_backward: null pointer");
     return ew_sum_backward(st, pgx, pgy, nrow, s);
+}
+
+// ---- decoder training ------------------------------------------------------------------------
+// The entry points from here on refuse bad arguments before they look for the device.
+static int no_host_path(int device) {
+    return device < 0 ? fail(KAI_E_NO_HOST_PATH, "device %d: this library has no CPU branch", device) : KAI_OK;
+}
+// Whether two buffers of that many floats share memory without being the same one.
+static bool partly_overlap(const float* a, int64_t na, const float* b, int64_t nb) {
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+    return a != nullptr && b != nullptr && pa != pb && pa < pb + 4 * static_cast<uintptr_t>(nb) &&
+           pb < pa + 4 * static_cast<uintptr_t>(na);
+}
+// The same, one buffer included.
+static bool share_memory(const float* a, int64_t na, const float* b, int64_t nb) {
+    return partly_overlap(a, na, b, nb) || (a != nullptr && a == b && na > 0 && nb > 0);
+}
+
+// ---- rotary positions -----------------------------------------------------------------------
+static int rotary_call(const char* name, int device, float* py, const float* px, const double* pfreq, const int64_t* ppos,
+                       int64_t pos0, int64_t nbat, int64_t ntimes, int64_t nhead, int64_t npiece, int64_t nrot, int layout,
+                       const float* scale, int64_t ldy, int64_t ldx, int backward, void* stream) {
+    KAI_TRY(no_host_path(device));
+    if (nbat < 0 || ntimes < 0 || nhead < 0 || npiece < 0) return fail(KAI_E_INVALID_ARG, "%s: negative extent", name);
+    if (nbat >= (int64_t(1) << 31) || ntimes >= (int64_t(1) << 31))
+        return fail(KAI_E_TOO_LARGE, "%s: 2^31 sequences or positions, or more", name);
+    if (nrot < 0 || nrot > npiece || (nrot & 1) != 0)
+        return fail(KAI_E_INVALID_ARG, "%s: nrot=%lld must be even and at most npiece", name, (long long)nrot);
+    if (layout != KAI_ROTARY_HALF && layout != KAI_ROTARY_INTERLEAVED)
+        return fail(KAI_E_INVALID_ARG, "%s: unknown layout %d", name, layout);
+    if (nhead >= (int64_t(1) << 31) || npiece >= (int64_t(1) << 31) || nhead * npiece >= (int64_t(1) << 31))
+        return fail(KAI_E_TOO_LARGE, "%s: a row has 2^31 values or more", name);
+    if (ldy < nhead * npiece || ldx < nhead * npiece)
+        return fail(KAI_E_INVALID_ARG, "%s: a row stride is shorter than nhead * npiece", name);
+    if (nbat * ntimes * nhead * npiece > 0 && (!py || !px || (!pfreq && nrot > 0)))
+        return fail(KAI_E_INVALID_ARG, "%s: null pointer", name);
+    if (py == px && ldy != ldx) return fail(KAI_E_INVALID_ARG, "%s: in place with two row strides", name);
+    const int64_t nvec = nhead * npiece;
+    if (ldy == nvec && ldx == nvec && partly_overlap(py, nbat * ntimes * nvec, px, nbat * ntimes * nvec))
+        return fail(KAI_E_INVALID_ARG, "%s: output and input overlap without being one buffer", name);
+    KAI_ENTER(device);
+    if (nbat * ntimes * nvec == 0) return KAI_OK;
+    return rotary(st, py, px, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot, layout, scale, ldy, ldx, backward, s);
+}
+
+int kai_rotary(int device, float* py, const float* px, const double* pfreq, const int64_t* ppos, int64_t pos0, int64_t nbat,
+               int64_t ntimes, int64_t nhead, int64_t npiece, int64_t nrot, int layout, const float* scale, int64_t ldy,
+               int64_t ldx, void* stream) {
+    return rotary_call("rotary", device, py, px, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot, layout, scale, ldy,
+                       ldx, 0, stream);
+}
+
+int kai_rotary_backward(int device, float* pgx, const float* pgy, const double* pfreq, const int64_t* ppos, int64_t pos0,
+                        int64_t nbat, int64_t ntimes, int64_t nhead, int64_t npiece, int64_t nrot, int layout,
+                        const float* scale, int64_t ldgx, int64_t ldgy, void* stream) {
+    return rotary_call("rotary_backward", device, pgx, pgy, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot, layout,
+                       scale, ldgx, ldgy, 1, stream);
+}
+
+int kai_rotary_frequencies(int device, double* pfreq, int64_t nrot, double base, int scaling, double factor, double slow,
+                           double fast, int64_t times, void* stream) {
+    KAI_TRY(no_host_path(device));
+    if (nrot < 0 || (nrot & 1) != 0 || nrot >= (int64_t(1) << 31))
+        return fail(KAI_E_INVALID_ARG, "rotary_frequencies: nrot must be even");
+    if (!(base > 0.0) || isinf(base)) return fail(KAI_E_INVALID_ARG, "rotary_frequencies: base must be positive");
+    if (scaling < KAI_ROTARY_PLAIN || scaling > KAI_ROTARY_BY_PARTS)
+        return fail(KAI_E_INVALID_ARG, "rotary_frequencies: unknown scaling %d", scaling);
+    if (scaling != KAI_ROTARY_PLAIN && (!(factor > 0.0) || isinf(factor)))
+        return fail(KAI_E_INVALID_ARG, "rotary_frequencies: factor must be positive");
+    if (scaling == KAI_ROTARY_BASE && nrot == 2)
+        return fail(KAI_E_INVALID_ARG, "rotary_frequencies: a single pair has no longest wavelength to stretch");
+    if (scaling == KAI_ROTARY_BY_PARTS && (!(slow >= 0.0) || !(fast > slow) || isinf(fast) || times <= 0))
+        return fail(KAI_E_INVALID_ARG, "rotary_frequencies: by parts needs 0 <= slow < fast and times > 0");
+    if (nrot > 0 && !pfreq) return fail(KAI_E_INVALID_ARG, "rotary_frequencies: null pointer");
+    KAI_ENTER(device);
+    (void)st;
+    if (nrot == 0) return KAI_OK;
+    return rotary_frequencies(pfreq, nrot, base, scaling, factor, slow, fast, times, s);
+}
+
+// ---- gated linear layer ---------------------------------------------------------------------
+static int gated_args(const char* name, int64_t yvec, int64_t ndat, int64_t xvec, int act) {
+    if (yvec < 0 || ndat < 0 || xvec < 0) return fail(KAI_E_INVALID_ARG, "%s: negative dimension", name);
+    const int64_t most = (int64_t(1) << 31) - 1;
+    if (yvec > most || ndat > most || xvec > most) return fail(KAI_E_TOO_LARGE, "%s: a dimension exceeds 2^31-1", name);
+    if (act < KAI_ACT_NONE || act > KAI_ACT_SWISH)
+        return fail(KAI_E_INVALID_ARG, "%s: activation %d is not elementwise", name, act);
+    return KAI_OK;
+}
+
+int kai_gated_linear_forward(int device, float* ph, float* pg, float* pu, const float* pwg, const float* pwu,
+                             const float* px, const float* pbg, const float* pbu, int64_t yvec, int64_t ndat, int64_t xvec,
+                             int act, const float* leaky_alpha, void* stream) {
+    KAI_TRY(no_host_path(device));
+    KAI_TRY(gated_args("gated_linear_forward", yvec, ndat, xvec, act));
+    if ((pg == nullptr) != (pu == nullptr))
+        return fail(KAI_E_INVALID_ARG, "gated_linear_forward: pg and pu are saved together or not at all");
+    if (ndat * yvec > 0 && (!ph || ((!pwg || !pwu || !px) && xvec > 0)))
+        return fail(KAI_E_INVALID_ARG, "gated_linear_forward: null pointer");
+    const int64_t nh = ndat * yvec;
+    if (share_memory(ph, nh, pg, nh) || share_memory(ph, nh, pu, nh) || share_memory(pg, nh, pu, nh) ||
+        share_memory(ph, nh, px, ndat * xvec) || share_memory(pg, nh, px, ndat * xvec) || share_memory(pu, nh, px, ndat * xvec))
+        return fail(KAI_E_INVALID_ARG, "gated_linear_forward: an output overlaps another output or px");
+    KAI_ENTER(device);
+    if (ndat == 0 || yvec == 0) return KAI_OK;
+    const int save = pg != nullptr;
+    if (!save) {
+        KAI_TRY(ensure_aux(st, 2 * ndat * yvec * 4));
+        pg = static_cast<float*>(st->aux);
+        pu = pg + ndat * yvec;
+    }
+    KAI_TRY(kai_sgemm(device, KAI_GEMM_NT, pg, px, pwg, ndat, yvec, xvec, yvec, 0, nullptr, KAI_ACT_NONE, nullptr,
+                      KAI_PATH_AUTO, stream));
+    KAI_TRY(kai_sgemm(device, KAI_GEMM_NT, pu, px, pwu, ndat, yvec, xvec, yvec, 0, nullptr, KAI_ACT_NONE, nullptr,
+                      KAI_PATH_AUTO, stream));
+    return gated_apply(st, ph, pg, pu, pbg, pbu, ndat, yvec, act, leaky_alpha, save, s);
+}
+
+int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float* pgwu, float* pgg, float* pgu, const float* pgh,
+                              const float* pg, const float* pu, const float* pwg, const float* pwu, const float* px,
+                              int64_t yvec, int64_t ndat, int64_t xvec, int act, const float* leaky_alpha, int acc_x,
+                              int acc_w, void* stream) {
+    KAI_TRY(no_host_path(device));
+    KAI_TRY(gated_args("gated_linear_backward", yvec, ndat, xvec, act));
+    if ((pgwg == nullptr) != (pgwu == nullptr))
+        return fail(KAI_E_INVALID_ARG, "gated_linear_backward: both weight gradients are wanted or none");
+    if (ndat * yvec > 0 && (!pgg || !pgu || !pgh || !pg || !pu))
+        return fail(KAI_E_INVALID_ARG, "gated_linear_backward: null pointer");
+    if (xvec > 0 && ((pgx && ndat * yvec > 0 && (!pwg || !pwu)) || (pgwg && ndat * yvec > 0 && !px)))
+        return fail(KAI_E_INVALID_ARG, "gated_linear_backward: null operand");
+    const int64_t nh = ndat * yvec, nx = ndat * xvec, nw = yvec * xvec;
+    bool clash = share_memory(pgg, nh, pgu, nh) || share_memory(pgwg, nw, pgwu, nw) || share_memory(pgg, nh, px, nx) ||
+                 share_memory(pgu, nh, px, nx);
+    for (const float* in : {pgh, pg, pu}) clash = clash || partly_overlap(pgg, nh, in, nh) || partly_overlap(pgu, nh, in, nh);
+    for (const float* w : {pwg, pwu, (const float*)pgwg, (const float*)pgwu}) clash = clash || share_memory(pgx, nx, w, nw);
+    for (const float* v : {(const float*)pgg, (const float*)pgu, px}) {
+        const int64_t n = v == px ? nx : nh;
+        clash = clash || share_memory(pgx, nx, v, n) || share_memory(pgwg, nw, v, n) || share_memory(pgwu, nw, v, n);
+    }
+    if (clash) return fail(KAI_E_INVALID_ARG, "gated_linear_backward: two buffers overlap");
+    KAI_ENTER(device);
+    if (ndat * yvec > 0)
+        KAI_TRY(gated_apply_backward(st, pgg, pgu, pgh, pg, pu, ndat * yvec, act, leaky_alpha, s));
+    if (pgx) {
+        KAI_TRY(kai_sgemm(device, KAI_GEMM_NN, pgx, pgg, pwg, ndat, xvec, yvec, xvec, acc_x, nullptr, KAI_ACT_NONE, nullptr,
+                          KAI_PATH_AUTO, stream));
+        KAI_TRY(kai_sgemm(device, KAI_GEMM_NN, pgx, pgu, pwu, ndat, xvec, yvec, xvec, 1, nullptr, KAI_ACT_NONE, nullptr,
+                          KAI_PATH_AUTO, stream));
+    }
+    if (pgwg) {
+        KAI_TRY(kai_sgemm(device, KAI_GEMM_TN, pgwg, pgg, px, yvec, xvec, ndat, xvec, acc_w, nullptr, KAI_ACT_NONE, nullptr,
+                          KAI_PATH_AUTO, stream));
+        KAI_TRY(kai_sgemm(device, KAI_GEMM_TN, pgwu, pgu, px, yvec, xvec, ndat, xvec, acc_w, nullptr, KAI_ACT_NONE, nullptr,
+                          KAI_PATH_AUTO, stream));
+    }
+    return KAI_OK;
+}
+
+// ---- losses on rows of logits ----------------------------------------------------------------
+static int row_loss_args(const char* name, int64_t nrow, int64_t ncol) {
+    if (nrow < 0 || ncol < 0) return fail(KAI_E_INVALID_ARG, "%s: negative extent", name);
+    if (ncol >= (int64_t(1) << 31)) return fail(KAI_E_TOO_LARGE, "%s: labels are 32-bit, ncol is not", name);
+    if (ncol == 0 && nrow > 0) return fail(KAI_E_INVALID_ARG, "%s: no columns", name);
+    return KAI_OK;
+}
+static int distill_args(const char* name, int64_t nrow, int64_t ncol, int64_t ntop) {
+    KAI_TRY(row_loss_args(name, nrow, ncol));
+    if (ntop < 0) return fail(KAI_E_INVALID_ARG, "%s: negative extent", name);
+    if (ntop > KAI_TOP_MAX) return fail(KAI_E_TOO_LARGE, "%s: ntop=%lld > %d", name, (long long)ntop, KAI_TOP_MAX);
+    return KAI_OK;
+}
+
+int kai_softmax_top_distill(int device, float* py, float* ps, const float* px, const int* pidx, const float* pt, int64_t nrow,
+                            int64_t ncol, int64_t ntop, const float* temp, void* stream) {
+    KAI_TRY(no_host_path(device));
+    KAI_TRY(distill_args("softmax_top_distill", nrow, ncol, ntop));
+    if (nrow > 0 && (!py || !ps || !px || (ntop > 0 && (!pidx || !pt))))
+        return fail(KAI_E_INVALID_ARG, "softmax_top_distill: null pointer");
+    KAI_ENTER(device);
+    if (nrow == 0) return KAI_OK;
+    return loss_distill(st, py, ps, px, pidx, pt, nrow, ncol, ntop, temp, s);
+}
+
+int kai_softmax_top_distill_backward_x(int device, float* pgx, const float* pgy, const float* px, const float* ps,
+                                       const int* pidx, const float* pt, int64_t nrow, int64_t ncol, int64_t ntop,
+                                       const float* temp, void* stream) {
+    KAI_TRY(no_host_path(device));
+    KAI_TRY(distill_args("softmax_top_distill_backward_x", nrow, ncol, ntop));
+    if (nrow > 0 && (!pgx || !px || !ps || (ntop > 0 && (!pidx || !pt))))
+        return fail(KAI_E_INVALID_ARG, "softmax_top_distill_backward_x: null pointer");
+    if (partly_overlap(pgx, nrow * ncol, px, nrow * ncol))
+        return fail(KAI_E_INVALID_ARG, "softmax_top_distill_backward_x: pgx and px overlap without being one buffer");
+    KAI_ENTER(device);
+    if (nrow == 0) return KAI_OK;
+    return loss_distill_backward(st, pgx, pgy, px, ps, pidx, pt, nrow, ncol, ntop, temp, s);
+}
+
+int kai_softmax_top_distill_step(int device, float* py, float* pgx, const float* pgy, const float* px, const int* pidx,
+                                 const float* pt, int64_t nrow, int64_t ncol, int64_t ntop, const float* temp,
+                                 void* stream) {
+    KAI_TRY(no_host_path(device));
+    KAI_TRY(distill_args("softmax_top_distill_step", nrow, ncol, ntop));
+    if (nrow > 0 && (!py || !pgx || !px || (ntop > 0 && (!pidx || !pt))))
+        return fail(KAI_E_INVALID_ARG, "softmax_top_distill_step: null pointer");
+    if (partly_overlap(pgx, nrow * ncol, px, nrow * ncol))
+        return fail(KAI_E_INVALID_ARG, "softmax_top_distill_step: pgx and px overlap without being one buffer");
+    KAI_ENTER(device);
+    if (nrow == 0) return KAI_OK;
+    return loss_distill_step(st, py, pgx, pgy, px, pidx, pt, nrow, ncol, ntop, temp, s);
+}
+
+int kai_softmax_policy_loss(int device, float* py, float* plogp, float* ps, const float* px, const int* pz,
+                            const float* pold, const float* pref, const float* padv, int64_t nrow, int64_t ncol,
+                            const float* clip_low, const float* clip_high, const float* kl_coef, const float* temp,
+                            void* stream) {
+    KAI_TRY(no_host_path(device));
+    KAI_TRY(row_loss_args("softmax_policy_loss", nrow, ncol));
+    if (nrow > 0 && (!py || !ps || !px || !pz || !padv))
+        return fail(KAI_E_INVALID_ARG, "softmax_policy_loss: null pointer");
+    KAI_ENTER(device);
+    if (nrow == 0) return KAI_OK;
+    return loss_policy(st, py, plogp, ps, px, pz, pold, pref, padv, nrow, ncol, clip_low, clip_high, kl_coef, temp, s);
+}
+
+int kai_softmax_policy_loss_backward_x(int device, float* pgx, const float* pgy, const float* px, const float* ps,
+                                       const int* pz, int64_t nrow, int64_t ncol, const float* temp, void* stream) {
+    KAI_TRY(no_host_path(device));
+    KAI_TRY(row_loss_args("softmax_policy_loss_backward_x", nrow, ncol));
+    if (nrow > 0 && (!pgx || !px || !ps || !pz))
+        return fail(KAI_E_INVALID_ARG, "softmax_policy_loss_backward_x: null pointer");
+    if (partly_overlap(pgx, nrow * ncol, px, nrow * ncol))
+        return fail(KAI_E_INVALID_ARG, "softmax_policy_loss_backward_x: pgx and px overlap without being one buffer");
+    KAI_ENTER(device);
+    if (nrow == 0) return KAI_OK;
+    return loss_policy_backward(st, pgx, pgy, px, ps, pz, nrow, ncol, temp, s);
+}
+
+int kai_softmax_policy_loss_step(int device, float* py, float* plogp, float* pgx, const float* pgy, const float* px,
+                                 const int* pz, const float* pold, const float* pref, const float* padv, int64_t nrow,
+                                 int64_t ncol, const float* clip_low, const float* clip_high, const float* kl_coef,
+                                 const float* temp, void* stream) {
+    KAI_TRY(no_host_path(device));
+    KAI_TRY(row_loss_args("softmax_policy_loss_step", nrow, ncol));
+    if (nrow > 0 && (!py || !pgx || !px || !pz || !padv))
+        return fail(KAI_E_INVALID_ARG, "softmax_policy_loss_step: null pointer");
+    if (partly_overlap(pgx, nrow * ncol, px, nrow * ncol))
+        return fail(KAI_E_INVALID_ARG, "softmax_policy_loss_step: pgx and px overlap without being one buffer");
+    KAI_ENTER(device);
+    if (nrow == 0) return KAI_OK;
+    return loss_policy_step(st, py, plogp, pgx, pgy, px, pz, pold, pref, padv, nrow, ncol, clip_low, clip_high, kl_coef,
+                            temp, s);
 }
 
 }  // extern "C"

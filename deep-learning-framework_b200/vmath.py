@@ -25,6 +25,13 @@ def _ptr(x):
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 
+def _typed(x, name):
+    """_ptr of an argument that is not fp32: a tensor of another type would be misread, not converted."""
+    if hasattr(x, "dtype") and str(x.dtype) != "torch." + name:
+        raise TypeError(f"a tensor of {name} is needed here, got {x.dtype}")
+    return _ptr(x)
+
+
 def _act(a) -> int:
     return capi.ACT[a] if isinstance(a, str) else int(a)
 
@@ -253,6 +260,81 @@ def sum(device, py, px, nrow, stream=None):  # noqa: A001 - the reference's name
 
 def sum_backward(device, pgx, pgy, nrow, stream=None):
     capi.call("kai_sum_backward", device, _ptr(pgx), _ptr(pgy), nrow, _ptr(stream))
+
+
+def rotary(device, py, px, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot, layout="half", hScale=None, ldy=None,
+           ldx=None, stream=None):
+    """Turns the pairs of every head by position * frequency; `layout` is "half" or "interleaved"."""
+    nvec = nhead * npiece
+    capi.call("kai_rotary", device, _ptr(py), _ptr(px), _typed(pfreq, "float64"), _typed(ppos, "int64"), pos0, nbat, ntimes,
+              nhead, npiece, nrot, capi.ROTARY_LAYOUT[layout], _ptr(hScale), nvec if ldy is None else ldy,
+              nvec if ldx is None else ldx, _ptr(stream))
+
+
+def rotary_backward(device, pgx, pgy, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot, layout="half", hScale=None,
+                    ldgx=None, ldgy=None, stream=None):
+    nvec = nhead * npiece
+    capi.call("kai_rotary_backward", device, _ptr(pgx), _ptr(pgy), _typed(pfreq, "float64"), _typed(ppos, "int64"), pos0,
+              nbat, ntimes, nhead, npiece, nrot, capi.ROTARY_LAYOUT[layout], _ptr(hScale), nvec if ldgx is None else ldgx,
+              nvec if ldgy is None else ldgy, _ptr(stream))
+
+
+def rotary_frequencies(device, pfreq, nrot, base=10000.0, scaling="plain", factor=1.0, slow=1.0, fast=32.0, times=1,
+                       stream=None):
+    """nrot / 2 doubles, radians per position; `scaling` is "plain", "linear", "base" or "by_parts"."""
+    capi.call("kai_rotary_frequencies", device, _typed(pfreq, "float64"), nrot, base, capi.ROTARY_SCALING[scaling], factor,
+              slow, fast, times, _ptr(stream))
+
+
+def gated_linear_forward(device, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act="swish", leaky_alpha=None,
+                         stream=None):
+    """ph = act(px . pwg^T + pbg) * (px . pwu^T + pbu); pg / pu receive the two factors' sums for the backward call."""
+    capi.call("kai_gated_linear_forward", device, _ptr(ph), _ptr(pg), _ptr(pu), _ptr(pwg), _ptr(pwu), _ptr(px), _ptr(pbg),
+              _ptr(pbu), yvec, ndat, xvec, _act(act), _ptr(leaky_alpha), _ptr(stream))
+
+
+def gated_linear_backward(device, pgx, pgwg, pgwu, pgg, pgu, pgh, pg, pu, pwg, pwu, px, yvec, ndat, xvec, act="swish",
+                          leaky_alpha=None, acc_x=False, acc_w=False, stream=None):
+    capi.call("kai_gated_linear_backward", device, _ptr(pgx), _ptr(pgwg), _ptr(pgwu), _ptr(pgg), _ptr(pgu), _ptr(pgh),
+              _ptr(pg), _ptr(pu), _ptr(pwg), _ptr(pwu), _ptr(px), yvec, ndat, xvec, _act(act), _ptr(leaky_alpha),
+              int(bool(acc_x)), int(bool(acc_w)), _ptr(stream))
+
+
+def softmax_top_distill(device, py, ps, px, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
+    """py[r] = temp^2 * KL(teacher's listed entries || softmax(px[r] / temp)); ps[nrow, 3] is for the backward call."""
+    capi.call("kai_softmax_top_distill", device, _ptr(py), _ptr(ps), _ptr(px), _typed(pidx, "int32"), _ptr(pt), nrow, ncol,
+              ntop, _ptr(hTemp), _ptr(stream))
+
+
+def softmax_top_distill_backward_x(device, pgx, pgy, px, ps, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
+    capi.call("kai_softmax_top_distill_backward_x", device, _ptr(pgx), _ptr(pgy), _ptr(px), _ptr(ps),
+              _typed(pidx, "int32"), _ptr(pt), nrow, ncol, ntop, _ptr(hTemp), _ptr(stream))
+
+
+def softmax_top_distill_step(device, py, pgx, pgy, px, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
+    """Loss and gradient with one read of the logits, for a pgy that is known beforehand (None: 1 for every row)."""
+    capi.call("kai_softmax_top_distill_step", device, _ptr(py), _ptr(pgx), _ptr(pgy), _ptr(px), _typed(pidx, "int32"),
+              _ptr(pt), nrow, ncol, ntop, _ptr(hTemp), _ptr(stream))
+
+
+def softmax_policy_loss(device, py, plogp, ps, px, pz, pold, pref, padv, nrow, ncol, hClipLow=None, hClipHigh=None,
+                        hKlCoef=None, hTemp=None, stream=None):
+    """Clipped policy loss of the tokens pz, with a KL term against pref; plogp receives their log-probabilities."""
+    capi.call("kai_softmax_policy_loss", device, _ptr(py), _ptr(plogp), _ptr(ps), _ptr(px), _typed(pz, "int32"), _ptr(pold),
+              _ptr(pref), _ptr(padv), nrow, ncol, _ptr(hClipLow), _ptr(hClipHigh), _ptr(hKlCoef), _ptr(hTemp), _ptr(stream))
+
+
+def softmax_policy_loss_backward_x(device, pgx, pgy, px, ps, pz, nrow, ncol, hTemp=None, stream=None):
+    capi.call("kai_softmax_policy_loss_backward_x", device, _ptr(pgx), _ptr(pgy), _ptr(px), _ptr(ps), _typed(pz, "int32"),
+              nrow, ncol, _ptr(hTemp), _ptr(stream))
+
+
+def softmax_policy_loss_step(device, py, plogp, pgx, pgy, px, pz, pold, pref, padv, nrow, ncol, hClipLow=None,
+                             hClipHigh=None, hKlCoef=None, hTemp=None, stream=None):
+    """Loss and gradient with one read of the logits, for a pgy that is known beforehand (None: 1 for every row)."""
+    capi.call("kai_softmax_policy_loss_step", device, _ptr(py), _ptr(plogp), _ptr(pgx), _ptr(pgy), _ptr(px),
+              _typed(pz, "int32"), _ptr(pold), _ptr(pref), _ptr(padv), nrow, ncol, _ptr(hClipLow), _ptr(hClipHigh),
+              _ptr(hKlCoef), _ptr(hTemp), _ptr(stream))
 
 
 class Replay:

@@ -418,6 +418,103 @@ KAI_API int kai_sum(int device, float* py, const float* px, int64_t nrow, void* 
 KAI_API int kai_sum_backward(int device, float* pgx, const float* pgy, int64_t nrow,
                              void* stream);
 
+/* ---- decoder training: rotary positions, gated linear layer, losses on logits ---------------
+ * No counterpart in the reference: what a decoder needs next to matmul, the attention trio and
+ * softmax_idx_crossentropy.  Same conventions as above (dense fp32 rows, HYPER pointers, `device`,
+ * `stream`); all of them are asynchronous and may be recorded. */
+
+/* Rotary positions.  The first nrot (even) of a head's npiece values form nrot / 2 pairs (a_i, b_i), which are turned
+ * by the angle pos * pfreq[i]:
+ *   a' = scale * (a cos - b sin),   b' = scale * (b cos + a sin);     the other npiece - nrot values are copied.
+ * layout KAI_ROTARY_HALF: a_i = head[i], b_i = head[i + nrot / 2];  KAI_ROTARY_INTERLEAVED: head[2i], head[2i + 1].
+ * px / py: nbat * ntimes rows of nhead * npiece floats, row strides ldx / ldy floats (>= nhead * npiece), so that the
+ * heads of a packed projection can be turned where they lie; py == px with ldy == ldx works in place, any other
+ * overlap of the two is not allowed.  pfreq: nrot / 2 doubles in device memory, radians per position.  ppos: one
+ * 64-bit position per row, or NULL: row (b, t) is at pos0 + t (pos0 is not used with ppos).  The angle is formed and
+ * reduced in 64 bits.  scale is a HYPER, except that NULL reads as 1.  The gradient is the rotation by the opposite
+ * angle, with the same scale. */
+#define KAI_ROTARY_HALF        0
+#define KAI_ROTARY_INTERLEAVED 1
+KAI_API int kai_rotary(int device, float* py, const float* px, const double* pfreq, const int64_t* ppos, int64_t pos0,
+                       int64_t nbat, int64_t ntimes, int64_t nhead, int64_t npiece, int64_t nrot, int layout,
+                       const float* scale, int64_t ldy, int64_t ldx, void* stream);
+KAI_API int kai_rotary_backward(int device, float* pgx, const float* pgy, const double* pfreq, const int64_t* ppos,
+                                int64_t pos0, int64_t nbat, int64_t ntimes, int64_t nhead, int64_t npiece, int64_t nrot,
+                                int layout, const float* scale, int64_t ldgx, int64_t ldgy, void* stream);
+/* Frequencies for the calls above: pfreq[i] = base^(-2i / nrot), then by `scaling`
+ *   KAI_ROTARY_PLAIN     as they are;
+ *   KAI_ROTARY_LINEAR    divided by factor (positions of a longer context squeezed into the trained one);
+ *   KAI_ROTARY_BASE      base replaced by base * factor^(nrot / (nrot - 2)): the longest wavelength grows by factor, the
+ *                        shortest stays (nrot > 2);
+ *   KAI_ROTARY_BY_PARTS  a pair that makes `fast` turns or more over the trained `times` positions keeps its frequency,
+ *                        one that makes `slow` or fewer is divided by factor, linear in the number of turns between.
+ * factor > 0, base > 0; slow, fast and times are only read by KAI_ROTARY_BY_PARTS (0 <= slow < fast, times > 0). */
+#define KAI_ROTARY_PLAIN    0
+#define KAI_ROTARY_LINEAR   1
+#define KAI_ROTARY_BASE     2
+#define KAI_ROTARY_BY_PARTS 3
+KAI_API int kai_rotary_frequencies(int device, double* pfreq, int64_t nrot, double base, int scaling, double factor,
+                                   double slow, double fast, int64_t times, void* stream);
+
+/* Gated linear layer:
+ *   g = px . pwg^T + pbg,   u = px . pwu^T + pbu,   ph[ndat,yvec] = act(g) * u
+ * with px[ndat,xvec], pwg / pwu[yvec,xvec]; pbg / pbu (length yvec) may be NULL, act is an elementwise KAI_ACT_*.
+ * pg / pu[ndat,yvec] receive g and u for the backward call; both NULL when none follows.
+ * Backward, from pgh (gradient of ph) and the saved pg / pu:
+ *   pgg = pgh * u * act'(g),   pgu = pgh * act(g)        (written; a bias gradient is kai_add_bias_backward_b of them)
+ *   pgx (+)= pgg . pwg + pgu . pwu,   pgwg (+)= pgg^T . px,   pgwu (+)= pgu^T . px
+ * acc_x / acc_w: += instead of =.  pgx may be NULL (input without gradient), and pgwg together with pgwu (fixed
+ * weights).  pgg and pgu may alias pg and pu, or pgh one of the two; other overlaps are not allowed. */
+KAI_API int kai_gated_linear_forward(int device, float* ph, float* pg, float* pu, const float* pwg, const float* pwu,
+                                     const float* px, const float* pbg, const float* pbu, int64_t yvec, int64_t ndat,
+                                     int64_t xvec, int act, const float* leaky_alpha, void* stream);
+KAI_API int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float* pgwu, float* pgg, float* pgu,
+                                      const float* pgh, const float* pg, const float* pu, const float* pwg,
+                                      const float* pwu, const float* px, int64_t yvec, int64_t ndat, int64_t xvec,
+                                      int act, const float* leaky_alpha, int acc_x, int acc_w, void* stream);
+
+/* Losses on rows of logits px[nrow,ncol], with q = softmax(px[r,:] / temp).  temp is a HYPER (> 0), except that NULL
+ * reads as 1.  Each comes as a forward call that saves three numbers per row in ps[nrow,3] (row maximum, sum of
+ * exponentials, d loss / d log-probability), a backward call that reads them, and a _step call that does both with one
+ * read of px, for callers that know the loss's gradient pgy[nrow] beforehand (NULL reads as 1 for every row).  pgx may
+ * be px itself in the backward and _step calls; any other overlap is not allowed.  Rows without a label
+ * (pz[r] = -1, or no used entry that has a weight) are padding: loss and gradient 0, whatever the logits hold.  Labels are checked on
+ * the device: any other label outside [0, ncol) makes the row's loss and gradient NaN and is reported by
+ * kai_device_status (KAI_E_OUT_OF_RANGE).
+ *
+ * Distillation from a teacher's top logits: pidx[nrow,ntop] names the columns, pt[nrow,ntop] holds the teacher's
+ * logits (or log-probabilities) there; unused entries have id -1, and an entry of -inf has no weight.  An id that
+ * occurs twice counts twice.  With p = softmax(pt[r,:] / temp) over the used entries,
+ *   py[r] = temp^2 * sum_j p_j * (log p_j - log q[pidx_j]);     ntop <= KAI_TOP_MAX
+ *   pgx[r,c] = pgy[r] * temp * (q_c - sum_{j: pidx_j = c} p_j) */
+#define KAI_TOP_MAX 2048
+KAI_API int kai_softmax_top_distill(int device, float* py, float* ps, const float* px, const int* pidx,
+                                    const float* pt, int64_t nrow, int64_t ncol, int64_t ntop, const float* temp,
+                                    void* stream);
+KAI_API int kai_softmax_top_distill_backward_x(int device, float* pgx, const float* pgy, const float* px,
+                                               const float* ps, const int* pidx, const float* pt, int64_t nrow,
+                                               int64_t ncol, int64_t ntop, const float* temp, void* stream);
+KAI_API int kai_softmax_top_distill_step(int device, float* py, float* pgx, const float* pgy, const float* px,
+                                         const int* pidx, const float* pt, int64_t nrow, int64_t ncol, int64_t ntop,
+                                         const float* temp, void* stream);
+/* Clipped policy loss with a KL term: with l = log q[pz[r]] and the ratio rho = exp(l - pold[r]),
+ *   py[r] = -min(rho * A, clip(rho, 1 - clip_low, 1 + clip_high) * A) + kl_coef * (e^d - d - 1),  A = padv[r], d = pref[r] - l
+ *   pgx[r,c] = pgy[r] / temp * dl * ([c = pz[r]] - q_c),   dl = -A * rho where the first term is the smaller or equal one
+ *              (else 0) + kl_coef * (1 - e^d)
+ * plogp[nrow] receives l (NULL: not wanted).  pold NULL: the sampling policy is the current one (rho = 1).  pref NULL:
+ * no KL term.  clip_low, clip_high, kl_coef are HYPERs; a NULL clip bound does not bound, a NULL kl_coef reads as 0. */
+KAI_API int kai_softmax_policy_loss(int device, float* py, float* plogp, float* ps, const float* px, const int* pz,
+                                    const float* pold, const float* pref, const float* padv, int64_t nrow, int64_t ncol,
+                                    const float* clip_low, const float* clip_high, const float* kl_coef,
+                                    const float* temp, void* stream);
+KAI_API int kai_softmax_policy_loss_backward_x(int device, float* pgx, const float* pgy, const float* px,
+                                               const float* ps, const int* pz, int64_t nrow, int64_t ncol,
+                                               const float* temp, void* stream);
+KAI_API int kai_softmax_policy_loss_step(int device, float* py, float* plogp, float* pgx, const float* pgy,
+                                         const float* px, const int* pz, const float* pold, const float* pref,
+                                         const float* padv, int64_t nrow, int64_t ncol, const float* clip_low,
+                                         const float* clip_high, const float* kl_coef, const float* temp, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
