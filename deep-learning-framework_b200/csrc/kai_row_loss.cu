@@ -1,53 +1,94 @@
 // Losses on rows of logits: distillation from a teacher's top logits, and the clipped policy loss with a KL term.
 //
 // Both are functions of log q at a few columns, q = softmax(x / T), and both have gradients of one form,
-//   gx_c = gy (k q_c - w_c),     w_c = 0 but for the columns named by the row's labels,
-//   distillation   k = T,          w = T p_j at column pidx_j              (p = softmax of the teacher's entries / T)
-//   policy         k = -dl / T,    w = -dl / T at column pz                (dl = d loss / d log q)
-// so they share three kernels, which differ only in a small description of the row (Distill / Policy below):
-//   row_loss_kernel   one read of the row with a running maximum and sum per thread; loss and the row's statistics
-//   row_grad_kernel   one read, one write, from the saved statistics
-//   row_step_kernel   loss and gradient with ONE read: the row stays in the registers of a cluster of CTAs
-// All are HBM-bound: 4, 8 and 8 bytes per logit.
+//   gx_c = k q_c - k w_c,     w_c = 0 but for the columns that the row's labels name,
+//   distillation   k = gy T,          w_c = sum of p_j with pidx_j = c        (p = softmax of the teacher's entries / T)
+//   policy         k = -gy dl / T,    w_c = 1 at c = pz                       (dl = d loss / d log q)
+// so they share their kernels, which differ only in a small description of a row's labels (Distill / Policy below).
 //
-// Precision: exponentials and their sums are fp32 (sums over at most a few hundred values per thread, then joined in
-// a fixed order); log q = (x - max) / T - log(sum) is formed in 64 bits per row, with the logarithm of the sum split into
-// exponent and mantissa: log(sum) rounded to fp32 would alone be off by up to 5e-7, which the ratio of two
-// probabilities and a clip bound next to it would see.
+// row_stream_kernel<L, T, MODE> is one persistent kernel for the three calls: kLoss (read the row: loss and
+// statistics), kGrad (read, write, from saved statistics) and kStep (loss and gradient with ONE read of the row).
+// All are HBM-bound: 4, 8 and 8 bytes per logit.
+//   * A row is spread over the shared memory of `parts` CTAs (kLoss, kStep: a cluster of 1 to 8): one bulk copy in, a pass for
+//     the maximum, a pass for the exponentials' sum, and (kStep, kGrad) a pass that turns the logits into the gradient
+//     in place, then one bulk copy out.  A CTA holds one part of one row; what hides its waits are the other
+//     CTAs of the SM, five or six parts of 32 KB.
+//   * Statistics: each warp takes its own reference and sum of exponentials and sends both to all CTAs of the row
+//     (distributed shared memory); ONE cluster barrier per row later every warp joins the same list in the same order.
+//   * Labels: a warp of its own prepares the next row's labels (teacher softmax, the student's logits at the ids) and parks
+//     what the row's loss is made of; eight parked rows are settled together, one per lane.
+// Measured on the way, 8192 x 32000, loss and gradient (2.1 GB, 320 us at the copy rate): row in registers, one CTA per
+// part and launch, 725 us; the same persistent, next rows fetched by cp.async, 640 us -- 21 instructions per value, most of
+// them addresses and bounds; by bulk copies, 657 us, the label warp's 13,000 clocks per row of 64-bit arithmetic now in
+// everybody's way; with the losses parked, 537 us.  There the registers still held the row (96 KB per SM) while twice
+// that lay prefetched in shared memory, and 8,000 clocks from load to store of each part bounded the rate; stores from
+// registers stood in the way of the label warp's loads.
+// row_loss_wide_kernel takes the rows that the shared memory of a cluster cannot hold (more than 400000 columns), for kLoss;
+// kStep is then kLoss and kGrad.
+//
+// Precision.  exp((x - m) / T) is formed as 2^(x c - k) with c = log2(e) / T rounded once and k the integer above m c: one
+// fused multiply-add, rounded relative to the exponent itself, and sums against different k are joined by exact powers of
+// two.  Rounding c is a temperature off by 2^-24, the same for every term.  Exponentials and their sums are fp32 (a few
+// dozen values per thread, then joined in a fixed order); log q = ln 2 (x c - k) - log(sum) is formed in 64 bits per row, with
+// the logarithm of the sum split into exponent and mantissa: log(sum) rounded to fp32 would alone be off by up to
+// 5e-7, which the ratio of two probabilities and a clip bound next to it would see.
 #include <math.h>
 
+#include <mutex>
+
 #include "kai_common.cuh"
+#include "kai_tcgen05.cuh"
 
 namespace kai {
 namespace {
 
-constexpr int kRowThreads = 512;
-constexpr int kRowWarps = kRowThreads / 32;
+enum Mode : int { kLoss, kGrad, kStep };
+
+// What a row's labels make of it.
+enum : int { kLive = 0, kPadding = 1, kBad = 2 };
+
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr int kMaxParts = 8;
+constexpr int kMaxWarps = 16;
 
 // ---- row geometry ----------------------------------------------------------------------------------
 // A row of any length at any 4-byte alignment is `head` scalars up to a 16-byte boundary, `quads` 16-byte pieces, and the
 // rest.  Part r of `parts` takes quads [r * per, (r + 1) * per); part 0 also takes the scalars, one for each of its first
 // threads.
 struct RowShape {
-    int64_t ncol, quads, per;
+    int quads, per;
     int head, loose;        // loose: scalars in front of and behind the quads, at most 6
-    __device__ __forceinline__ RowShape(const float* x, int64_t ncol_, int parts) {
-        ncol = ncol_;
+    // per_: pieces of a part, the same for all rows (the alignment of a row costs at most one piece)
+    __device__ __forceinline__ RowShape(const float* x, int ncol, int per_) : per(per_) {
         head = static_cast<int>((4 - ((reinterpret_cast<uintptr_t>(x) >> 2) & 3)) & 3);
-        if (head > ncol) head = static_cast<int>(ncol);
+        if (head > ncol) head = ncol;
         quads = (ncol - head) >> 2;
-        loose = static_cast<int>(ncol - 4 * quads);
-        per = (quads + parts - 1) / parts;
+        loose = ncol - 4 * quads;
     }
-    __device__ __forceinline__ int64_t loose_col(int i) const { return i < head ? i : 4 * quads + i; }
-    __device__ __forceinline__ bool owned(int64_t c, int part) const {
-        const int64_t q = (c - head) >> 2;
+    __device__ __forceinline__ int begin(int part) const { return min(part * per, quads); }
+    __device__ __forceinline__ int count(int part) const { return min(per, quads - begin(part)); }
+    __device__ __forceinline__ int loose_col(int i) const { return i < head ? i : 4 * quads + i; }
+    __device__ __forceinline__ bool owned(int c, int part) const {
+        const int q = (c - head) >> 2;
         if (c < head || q >= quads) return part == 0;
-        return q >= part * per && q < (part + 1) * per;
+        return q >= begin(part) && q < begin(part) + per;
     }
 };
 
-__device__ __forceinline__ void max4(const float4& v, float& m) { m = fmaxf(fmaxf(m, fmaxf(v.x, v.y)), fmaxf(v.z, v.w)); }
+__device__ __forceinline__ float max4(const float4& v, float m) {
+    return fmaxf(fmaxf(m, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+}
+__device__ __forceinline__ float warp_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+template <class V>
+__device__ __forceinline__ V warp_sum(V v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
 // log of a positive sum, to about 1e-8 absolute
 __device__ __forceinline__ double log_sum(float s) {
@@ -55,165 +96,220 @@ __device__ __forceinline__ double log_sum(float s) {
     int e;
     float f = frexpf(s, &e);
     if (f < 0.70710678f) { f *= 2.0f; --e; }
-    return e * 0.69314718055994530942 + static_cast<double>(logf(f));
+    return e * kLn2 + static_cast<double>(logf(f));
 }
 
-// Block-wide maximum / sum, the same value in every thread; `red` holds one float per warp.
-__device__ __forceinline__ float block_max(float v, float* red) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[threadIdx.x & (kRowWarps - 1)];
-#pragma unroll
-    for (int o = kRowWarps / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+// 2^(x c - k).  Against k = -inf (nothing but -inf was seen) the caller uses 0, so that -inf has no weight instead of
+// being NaN.
+__device__ __forceinline__ float exp2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
-__device__ __forceinline__ float block_sum(float v, float* red) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[threadIdx.x & (kRowWarps - 1)];
-#pragma unroll
-    for (int o = kRowWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+__device__ __forceinline__ float weight(float x, float k, float c) { return exp2_approx(fmaf(x, c, -k)); }
+__device__ __forceinline__ float reference(float m, float c) { return ceilf(m * c); }
+__device__ __forceinline__ float finite_ref(float k) { return k == -INFINITY ? 0.0f : k; }
+__device__ __forceinline__ float weight4(float4 v, float k, float c) {
+    v = make_float4(weight(v.x, k, c), weight(v.y, k, c), weight(v.z, k, c), weight(v.w, k, c));
+    return (v.x + v.y) + (v.z + v.w);
 }
+struct RowParams {
+    const float* x;
+    float* y;
+    float* ps;
+    float* gx;
+    const float* gy;
+    const float* temp;
+    int64_t nrow, ncol;
+    int parts;       // CTAs per row
+    int per;         // 16-byte pieces of a part, and of a stage
+    int* flag;       // label outside its range
+    int* status;     // a bounded wait ran out
+};
 
-// exp((x - m) / T); a part of a row that holds nothing but -inf has m = -inf and no weight
-__device__ __forceinline__ float weight(float x, float m, float inv_t) {
-    return (m == -INFINITY && x == -INFINITY) ? 0.0f : expf((x - m) * inv_t);
-}
+// What both kinds of labels keep of a row in shared memory.
+struct alignas(16) RowHead {
+    float gy;
+    float stat[3];           // the saved row of ps (kGrad): reference, sum, slope
+    int state;
+    float teacher, weights;  // distillation: reference and sum of the teacher's weights
+};
+constexpr int kParked = 8;  // rows whose losses are settled together
+static_assert(sizeof(RowHead) % 16 == 0, "what follows it in shared memory is read 16 bytes at a time");
 
-// What a row's labels make of it.
-enum : int { kLive = 0, kPadding = 1, kBad = 2 };
+struct Temp {
+    float t, c;       // temperature, log2(e) / T
+    __device__ __forceinline__ explicit Temp(const float* p) {
+        t = (p != nullptr) ? __ldg(p) : 1.0f;
+        c = static_cast<float>(1.44269504088896340736 / static_cast<double>(t));
+    }
+    // log2 of the weight of x against k
+    __device__ __forceinline__ double exponent(float x, float k) const {
+        return static_cast<double>(x) * static_cast<double>(c) - static_cast<double>(k);
+    }
+};
 
-struct RowResult {
-    float loss;
-    float slope;   // d loss / d log q, without gy (distillation: the p_j carry the labels, slope is 1)
-    float logp;
+struct Result {
+    float loss, slope, logp;     // slope: d loss / d log q, without gy (distillation: the p_j carry the labels, slope is 1)
 };
 
 // ---- distillation ------------------------------------------------------------------------------------
 struct Distill {
     const int* idx;
     const float* t;
-    const float* temp;
-    int ntop;
+    int ntop, ntop4;       // ntop4: rounded up to a multiple of 4, unused entries behind ntop
 
-    // Shared memory of a row: the ids, the teacher's weights, and the student's logits there.
-    struct Smem {
-        int* id;        // [ntop] column, -1 = unused; `first` marks the entry that speaks for repeated ids
-        float* p;       // [ntop] probability of the entry
-        float* sum;     // [ntop] probability of all entries with that id (first occurrence), negative elsewhere
-        float* xz;      // [ntop] logit of the student
-        float* scalar;  // [0] sum of teacher weights
-        int* state;
-    };
-    static __host__ __device__ size_t smem_bytes(int ntop) { return 16 * static_cast<size_t>(ntop) + 16; }
-    __device__ __forceinline__ Smem smem(uint8_t* base) const {
-        Smem m;
-        m.id = reinterpret_cast<int*>(base);
-        m.p = reinterpret_cast<float*>(m.id + ntop);
-        m.sum = m.p + ntop;
-        m.xz = m.sum + ntop;
-        m.scalar = m.xz + ntop;
-        m.state = reinterpret_cast<int*>(m.scalar + 2);
-        return m;
-    }
-    __device__ __forceinline__ float temperature() const { return temp != nullptr ? __ldg(temp) : 1.0f; }
-
-    // Step 1 (before the first block-wide barrier): ids, and what the student says there.  Every thread, strided.
-    __device__ __forceinline__ void gather(const Smem& m, const float* x, int64_t row, int64_t ncol) const {
-        for (int j = threadIdx.x; j < ntop; j += kRowThreads) {
-            const int id = idx[row * ntop + j];
-            m.id[j] = id;
-            m.p[j] = t[row * ntop + j];
-            m.xz[j] = (x != nullptr && id >= 0 && id < ncol) ? x[id] : 0.0f;
-        }
-    }
-    // Step 2 (after a barrier): warp 0 turns the teacher's entries into probabilities.  p = 0 for unused entries.
-    __device__ __forceinline__ void teacher(const Smem& m, int64_t ncol) const {
-        if (threadIdx.x >= 32) return;
-        const int lane = threadIdx.x;
-        const float inv_t = 1.0f / temperature();
-        float top = -INFINITY;
-        bool bad = false, some = false, nan = false;
-        for (int j = lane; j < ntop; j += 32) {
-            const int id = m.id[j];
-            if (id < -1 || id >= ncol) bad = true;
-            if (id >= 0) {
-                some = some || m.p[j] > -INFINITY;
-                nan = nan || isnan(m.p[j]);
-                top = fmaxf(top, m.p[j]);
-            }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        bad = __any_sync(0xffffffffu, bad);
-        some = __any_sync(0xffffffffu, some || nan);
-        float sum = 0.0f;
-        for (int j = lane; j < ntop; j += 32) {
-            const float e = (m.id[j] >= 0 && some) ? expf((m.p[j] - top) * inv_t) : 0.0f;
-            sum += e;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = 1.0f / sum;
-        // the logit makes room for the probability; its logarithm is formed again from that logit, so keep it in `sum`
-        for (int j = lane; j < ntop; j += 32) {
-            const float v = m.p[j];
-            m.sum[j] = (v - top) * inv_t;
-            m.p[j] = (m.id[j] >= 0 && some) ? expf((v - top) * inv_t) * inv : 0.0f;
-        }
-        if (lane == 0) {
-            m.scalar[0] = sum;
-            *m.state = bad ? kBad : (some ? kLive : kPadding);
-        }
-    }
-    __device__ __forceinline__ int state(const Smem& m) const { return *m.state; }
-
-    // Step 3 (after a barrier, statistics known; one warp): the loss.
-    __device__ __forceinline__ RowResult finish(const Smem& m, float top, float total, int64_t) const {
-        const float tv = temperature();
-        const float inv_t = 1.0f / tv;
-        double s = 0.0;
-        for (int j = threadIdx.x & 31; j < ntop; j += 32) {
-            const float p = m.p[j];
-            if (p != 0.0f)   // NaN included
-                s += static_cast<double>(p) * (static_cast<double>(m.sum[j]) -
-                                               (static_cast<double>(m.xz[j]) - static_cast<double>(top)) * inv_t);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s += log_sum(total) - log_sum(m.scalar[0]);
-        RowResult r;
-        r.loss = static_cast<float>(static_cast<double>(tv) * tv * s);
-        r.slope = 1.0f;
-        r.logp = 0.0f;
-        return r;
-    }
-    // Step 4 (after a barrier): one entry speaks for all that name the same column.  Overwrites `sum`.
-    __device__ __forceinline__ void merge(const Smem& m) const {
-        for (int j = threadIdx.x; j < ntop; j += kRowThreads) {
-            const int id = m.id[j];
-            float sum = 0.0f;
-            bool first = id >= 0;
-            for (int i = 0; i < ntop; ++i) {
-                const bool same = m.id[i] == id;
-                if (same && i < j) first = false;
-                if (same) sum += m.p[i];
-            }
-            m.sum[j] = first ? sum : -1.0f;
-        }
-    }
-    // gx = gy T (q - sum p)
-    __device__ __forceinline__ float q_coef(float gy, float) const { return gy * temperature(); }
+    struct Row : RowHead {};
+    __host__ __device__ size_t bytes() const { return sizeof(RowHead) + 16 * static_cast<size_t>(ntop4); }
+    static __device__ __forceinline__ int* ids(Row* r) { return reinterpret_cast<int*>(r + 1); }
+    __device__ __forceinline__ float* probs(Row* r) const { return reinterpret_cast<float*>(ids(r) + ntop4); }
+    __device__ __forceinline__ float* logits(Row* r) const { return probs(r) + ntop4; }
+    __device__ __forceinline__ float* teacher(Row* r) const { return logits(r) + ntop4; }
     __device__ __forceinline__ int labels() const { return ntop; }
-    __device__ __forceinline__ bool label(const Smem& m, int j, int64_t& c, float& w) const {
-        c = m.id[j];
-        w = m.sum[j];
-        return w >= 0.0f || isnan(w);
+
+    // The label warp works ahead so that no load of its own is waited for: ids and teacher logits are fetched two rows ahead
+    // (Ahead), the student's logits there one row ahead (Flight), up to kAhead labels per lane; what is beyond is loaded in
+    // place.
+    static constexpr int kAhead = 4;
+    struct Ahead {
+        int id[kAhead];
+        float t[kAhead];
+    };
+    struct Flight {
+        float x[kAhead];
+    };
+    __device__ __forceinline__ void ahead(Ahead& a, int64_t row) const {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int j = (threadIdx.x & 31) + 32 * i;
+            a.id[i] = j < ntop ? idx[row * ntop + j] : -1;
+            a.t[i] = j < ntop ? t[row * ntop + j] : 0.0f;
+        }
+    }
+    // The student's logits at ids of this part, or at all of them.
+    __device__ __forceinline__ void depart(Flight& f, const Ahead& a, const float* x, const RowShape& shape, int part, bool all,
+                                           int64_t, int64_t ncol) const {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int z = a.id[i];
+            f.x[i] = (z >= 0 && z < ncol && (all || shape.owned(z, part))) ? x[z] : 0.0f;
+        }
+    }
+    // One warp: labels and logits into shared memory, the teacher's entries as probabilities (0 for unused entries), and
+    // the row's state.
+    __device__ __forceinline__ void arrive(Row* r, const Flight& f, const Ahead& a, const float* x, const RowShape& shape,
+                                           int part, bool all, int64_t row, int64_t ncol, const Temp& tv) const {
+        const int lane = threadIdx.x & 31;
+        int* id = ids(r);
+        float* p = probs(r);
+        float* xz = logits(r);
+        float* te = teacher(r);
+        float top = -INFINITY;
+        bool bad = false, some = false;
+        auto take = [&](int j, int z, float v, float xv) {
+            id[j] = z;
+            te[j] = v;
+            xz[j] = xv;
+            if (z < -1 || z >= ncol) bad = true;
+            if (z >= 0) {
+                some = some || !(v == -INFINITY);      // NaN counts: it poisons the row
+                top = fmaxf(top, v);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (lane + 32 * i < ntop4) take(lane + 32 * i, a.id[i], a.t[i], f.x[i]);
+#pragma unroll 4
+        for (int j = lane + 32 * kAhead; j < ntop4; j += 32) {
+            const int z = j < ntop ? idx[row * ntop + j] : -1;
+            const bool read = z >= 0 && z < ncol && (all || shape.owned(z, part));
+            take(j, z, j < ntop ? t[row * ntop + j] : 0.0f, read ? x[z] : 0.0f);
+        }
+        top = warp_max(top);
+        bad = __any_sync(0xffffffffu, bad);
+        some = __any_sync(0xffffffffu, some);
+        const float k = finite_ref(reference(top, tv.c));
+        float sum = 0.0f;
+        for (int j = lane; j < ntop4; j += 32) {
+            const float e = (id[j] >= 0) ? weight(te[j], k, tv.c) : 0.0f;
+            sum += e;
+            p[j] = e;
+        }
+        sum = warp_sum(sum);
+        const float inv = some ? 1.0f / sum : 0.0f;
+        for (int j = lane; j < ntop4; j += 32) p[j] *= inv;
+        if (lane == 0) {
+            r->teacher = k;
+            r->weights = sum;
+            r->state = bad ? kBad : (some ? kLive : kPadding);
+        }
+    }
+    // What the loss of a row is made of: loss = T^2 (ln 2 sum_j p_j (log2-weight of the teacher - of the student) + log S - log W).
+    // Each lane leaves its part of the sum.
+    struct Parked {
+        double part[kParked][33];
+        float k[kParked], total[kParked], weights[kParked];
+        int state[kParked];
+    };
+    __device__ __forceinline__ void park(Parked* q, int slot, Row* r, float k, float total, const Temp& tv) const {
+        const int lane = threadIdx.x & 31;
+        const double shift = static_cast<double>(r->teacher) - static_cast<double>(finite_ref(k));
+        double s = 0.0;
+        for (int j = lane; j < ntop; j += 32) {
+            const float p = probs(r)[j];
+            if (p != 0.0f)
+                s += static_cast<double>(p) *
+                     ((static_cast<double>(teacher(r)[j]) - static_cast<double>(logits(r)[j])) * static_cast<double>(tv.c) - shift);
+        }
+        q->part[slot][lane] = s;
+        if (lane == 0) {
+            q->k[slot] = k; q->total[slot] = total; q->weights[slot] = r->weights; q->state[slot] = r->state;
+        }
+    }
+    __device__ __forceinline__ Result settle(const Parked* q, int slot, const Temp& tv) const {
+        double s = 0.0;
+#pragma unroll 4
+        for (int i = 0; i < 32; ++i) s += q->part[slot][i];
+        s = kLn2 * s + log_sum(q->total[slot]) - log_sum(q->weights[slot]);
+        return Result{static_cast<float>(static_cast<double>(tv.t) * tv.t * s), 1.0f, 0.0f};
+    }
+    __device__ __forceinline__ float finish_slope(Row*, float, float, const Temp&) const { return 1.0f; }
+    __device__ __forceinline__ float coef(Row* r, float, const Temp& tv) const { return r->gy * tv.t; }
+    // Threads that share the search for one label's repetitions: a power of two up to 32, `threads` being a multiple of 32.
+    __device__ __forceinline__ int sharers(int threads) const {
+        int g = 1;
+        while (g < 32 && 2 * g * ntop <= threads) g *= 2;
+        return g;
+    }
+    // Label j's column and weight; an id that occurs again belongs to its first place.  Called by whole warps: thread `sub` of
+    // `g` neighbours looks through every g-th group of four entries, in an order that g alone determines.
+    __device__ __forceinline__ bool label(Row* r, int j, int sub, int g, int& c, float& w, float& x) const {
+        const int z = j < ntop ? ids(r)[j] : -1;
+        int first = j;
+        float sum = 0.0f;
+        if (z >= 0) {
+            const int4* id4 = reinterpret_cast<const int4*>(ids(r));
+            const float4* p4 = reinterpret_cast<const float4*>(probs(r));
+#pragma unroll 4
+            for (int i = sub; i < ntop4 / 4; i += g) {
+                const int4 v = id4[i];
+                if (v.x == z || v.y == z || v.z == z || v.w == z) {
+                    const float4 q = p4[i];
+                    if (v.x == z) { sum += q.x; first = min(first, 4 * i); }
+                    if (v.y == z) { sum += q.y; first = min(first, 4 * i + 1); }
+                    if (v.z == z) { sum += q.z; first = min(first, 4 * i + 2); }
+                    if (v.w == z) { sum += q.w; first = min(first, 4 * i + 3); }
+                }
+            }
+            x = logits(r)[j];
+        }
+        for (int o = 1; o < g; o *= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+        }
+        c = z;
+        w = sum;
+        return z >= 0 && first == j && sub == 0;
     }
     __device__ __forceinline__ void extra(int64_t, float) const {}
 };
@@ -227,34 +323,43 @@ struct Policy {
     const float* low;
     const float* high;
     const float* beta;
-    const float* temp;
     float* logp;
 
-    struct Smem {
-        int* id;
-        float* xz;
-        int* state;
+    // The label warp's pipeline, as above: the token two rows ahead, what belongs to it one row ahead.
+    struct Ahead {
+        int id;
     };
-    static __host__ __device__ size_t smem_bytes(int) { return 16; }
-    __device__ __forceinline__ Smem smem(uint8_t* base) const {
-        return Smem{reinterpret_cast<int*>(base), reinterpret_cast<float*>(base) + 1, reinterpret_cast<int*>(base) + 2};
+    struct Flight {
+        float x, old, ref, adv;
+    };
+
+    struct Row : RowHead {
+        Flight token;
+        int id;
+    };
+    __host__ __device__ size_t bytes() const { return sizeof(Row); }
+    __device__ __forceinline__ int labels() const { return 1; }
+
+    __device__ __forceinline__ void ahead(Ahead& a, int64_t row) const { a.id = z[row]; }
+    __device__ __forceinline__ void depart(Flight& f, const Ahead& a, const float* x, const RowShape& shape, int part, bool all,
+                                           int64_t row, int64_t ncol) const {
+        f.x = (a.id >= 0 && a.id < ncol && (all || shape.owned(a.id, part))) ? x[a.id] : 0.0f;
+        f.old = (old_logp != nullptr) ? old_logp[row] : 0.0f;
+        f.ref = (ref_logp != nullptr) ? ref_logp[row] : 0.0f;
+        f.adv = (adv != nullptr) ? adv[row] : 0.0f;
     }
-    __device__ __forceinline__ float temperature() const { return temp != nullptr ? __ldg(temp) : 1.0f; }
-    __device__ __forceinline__ void gather(const Smem& m, const float* x, int64_t row, int64_t ncol) const {
-        if (threadIdx.x == 0) {
-            const int id = z[row];
-            const bool in = id >= 0 && id < ncol;
-            *m.id = id;
-            *m.state = in ? kLive : (id == -1 ? kPadding : kBad);
-            *m.xz = (x != nullptr && in) ? x[id] : 0.0f;
+    __device__ __forceinline__ void arrive(Row* r, const Flight& f, const Ahead& a, const float*, const RowShape&, int, bool,
+                                           int64_t, int64_t ncol, const Temp&) const {
+        if ((threadIdx.x & 31) == 0) {
+            r->id = a.id;
+            r->state = (a.id >= 0 && a.id < ncol) ? kLive : (a.id == -1 ? kPadding : kBad);
+            r->token = f;
         }
     }
-    __device__ __forceinline__ void teacher(const Smem&, int64_t) const {}
-    __device__ __forceinline__ int state(const Smem& m) const { return *m.state; }
-    __device__ __forceinline__ RowResult finish(const Smem& m, float top, float total, int64_t row) const {
-        const double l = (static_cast<double>(*m.xz) - static_cast<double>(top)) / temperature() - log_sum(total);
-        const float a = adv[row];
-        const float rho = (old_logp != nullptr) ? expf(static_cast<float>(l - static_cast<double>(old_logp[row]))) : 1.0f;
+    __device__ __forceinline__ Result finish(const Flight& v, float k, float total, const Temp& tv) const {
+        const double l = kLn2 * tv.exponent(v.x, finite_ref(k)) - log_sum(total);
+        const float a = v.adv;
+        const float rho = (old_logp != nullptr) ? expf(static_cast<float>(l - static_cast<double>(v.old))) : 1.0f;
         float bound = rho;
         if (low != nullptr) bound = fmaxf(bound, 1.0f - __ldg(low));
         if (high != nullptr) bound = fminf(bound, 1.0f + __ldg(high));
@@ -263,48 +368,53 @@ struct Policy {
         const float ra = (a == 0.0f && !isnan(rho)) ? 0.0f : rho * a;
         const float ba = (a == 0.0f) ? 0.0f : bound * a;
         const bool free = !(ra > ba);
-        RowResult r;
-        r.loss = free ? -ra : -ba;
-        r.slope = free ? -ra : 0.0f;
+        Result out;
+        out.loss = free ? -ra : -ba;
+        out.slope = free ? -ra : 0.0f;
         if (ref_logp != nullptr && beta != nullptr) {
             const float b = __ldg(beta);
-            const float d = static_cast<float>(static_cast<double>(ref_logp[row]) - l);
+            const float d = static_cast<float>(static_cast<double>(v.ref) - l);
             const float e1 = expm1f(d);          // e^d - 1: the term is d^2 / 2 next to 0, e^d - d - 1 would cancel
-            r.loss = fmaf(b, e1 - d, r.loss);
-            r.slope = fmaf(-b, e1, r.slope);
+            out.loss = fmaf(b, e1 - d, out.loss);
+            out.slope = fmaf(-b, e1, out.slope);
         }
-        r.logp = static_cast<float>(l);
-        return r;
+        out.logp = static_cast<float>(l);
+        return out;
     }
-    __device__ __forceinline__ void merge(const Smem&) const {}
-    __device__ __forceinline__ float q_coef(float gy, float slope) const { return -(gy * slope) / temperature(); }
-    __device__ __forceinline__ int labels() const { return 1; }
-    __device__ __forceinline__ bool label(const Smem& m, int, int64_t& c, float& w) const {
-        c = *m.id;
+    // kGrad brings the saved slope; kStep works it out in every warp, which spares a second barrier.
+    __device__ __forceinline__ float finish_slope(Row* r, float k, float total, const Temp& tv) const {
+        return finish(r->token, k, total, tv).slope;
+    }
+    __device__ __forceinline__ float coef(Row* r, float slope, const Temp& tv) const {
+        return -(r->gy * slope) / tv.t;
+    }
+    __device__ __forceinline__ int sharers(int) const { return 1; }
+    __device__ __forceinline__ bool label(Row* r, int j, int, int, int& c, float& w, float& x) const {
+        c = r->id;
         w = 1.0f;
-        return true;
+        x = r->token.x;
+        return j == 0;
+    }
+    struct Parked {
+        Flight token[kParked];
+        float k[kParked], total[kParked];
+        int state[kParked];
+    };
+    __device__ __forceinline__ void park(Parked* q, int slot, Row* r, float k, float total, const Temp&) const {
+        if ((threadIdx.x & 31) == 0) {
+            q->token[slot] = r->token;
+            q->k[slot] = k; q->total[slot] = total; q->state[slot] = r->state;
+        }
+    }
+    __device__ __forceinline__ Result settle(const Parked* q, int slot, const Temp& tv) const {
+        return finish(q->token[slot], q->k[slot], q->total[slot], tv);
     }
     __device__ __forceinline__ void extra(int64_t row, float v) const {
         if (logp != nullptr) logp[row] = v;
     }
 };
 
-struct RowParams {
-    const float* x;
-    float* y;
-    float* ps;
-    float* gx;
-    const float* gy;
-    int64_t ncol;
-    int parts;       // CTAs per row
-    int* flag;
-};
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
+// ---- clusters ------------------------------------------------------------------------------------------
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Writes two floats to the same shared-memory variable of CTA `rank` of the cluster.
@@ -314,260 +424,369 @@ __device__ __forceinline__ void push_stat(float2* local, uint32_t rank, float a,
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(a), "f"(b) : "memory");
 }
-
-// Joins the parts' (maximum, sum of exponentials against it).  Rank order, the same in every CTA.
-__device__ __forceinline__ void join(const float2* stat, int parts, float inv_t, float& top, float& total) {
-    top = stat[0].x;
-    for (int i = 1; i < parts; ++i) top = fmaxf(top, stat[i].x);
-    total = 0.0f;
-    for (int i = 0; i < parts; ++i) total += stat[i].y * weight(stat[i].x, top, inv_t);
+// `bytes` (a multiple of 16, both addresses on 16-byte boundaries) into shared memory; the barrier is credited as they land.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
-// ---- loss alone ------------------------------------------------------------------------------------------
-// A thread keeps a running maximum m and sum s over its pieces of the row, four 16-byte loads at a time: the maximum of
-// the sixteen values first, one rescaling of s if it rose, then sixteen exponentials.
-template <class L>
-__global__ void __launch_bounds__(kRowThreads)
-row_loss_kernel(const RowParams p, const L loss) {
-    extern __shared__ __align__(16) uint8_t dyn[];
-    __shared__ float red_m[kRowWarps], red_s[kRowWarps];
-    __shared__ float2 stat[8];
-    const int64_t row = blockIdx.x / p.parts;
-    const int part = blockIdx.x % p.parts;
-    if (p.parts > 1) cluster_arrive();
-    const float* x = p.x + row * p.ncol;
-    const RowShape shape(x, p.ncol, p.parts);
-    const typename L::Smem sm = loss.smem(dyn);
-    const float inv_t = 1.0f / loss.temperature();
-    if (part == 0) loss.gather(sm, x, row, p.ncol);
-
-    const float4* xq = reinterpret_cast<const float4*>(x + shape.head);
-    const int64_t q_end = min(shape.quads, (part + 1) * shape.per);
-    float m = -INFINITY, s = 0.0f;
-    for (int64_t q0 = part * shape.per + threadIdx.x; q0 < q_end; q0 += 4 * kRowThreads) {
-        float4 v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int64_t q = q0 + u * kRowThreads;
-            v[u] = (q < q_end) ? __ldcs(xq + q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        }
-        float m1 = m;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) max4(v[u], m1);
-        if (m1 > m) { s *= weight(m, m1, inv_t); m = m1; }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            s += (weight(v[u].x, m, inv_t) + weight(v[u].y, m, inv_t)) + (weight(v[u].z, m, inv_t) + weight(v[u].w, m, inv_t));
-    }
-    if (part == 0 && static_cast<int>(threadIdx.x) < shape.loose) {
-        const float v = x[shape.loose_col(threadIdx.x)];
-        if (v > m) { s *= weight(m, v, inv_t); m = v; }
-        s += weight(v, m, inv_t);
-    }
-    float top = block_max(m, red_m);
-    if (part == 0) loss.teacher(sm, p.ncol);
-    float total = block_sum(s * weight(m, top, inv_t), red_s);
-    if (p.parts > 1) {
-        cluster_wait();                         // every CTA of the cluster has begun
-        if (threadIdx.x == 0) push_stat(&stat[part], 0, top, total);
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-        if (part != 0) return;
-        join(stat, p.parts, inv_t, top, total);
-    }
-    if (threadIdx.x < 32) {
-        const int state = loss.state(sm);
-        RowResult r = loss.finish(sm, top, total, row);
-        if (state == kPadding) r.loss = r.slope = r.logp = 0.0f;
-        if (state == kBad) r.loss = r.slope = r.logp = nanf("");
-        if (threadIdx.x == 0) {
-            p.y[row] = r.loss;
-            loss.extra(row, r.logp);
-            p.ps[3 * row + 0] = top;
-            p.ps[3 * row + 1] = total;
-            p.ps[3 * row + 2] = r.slope;
-            if (state == kBad) *p.flag = 1;
-        }
-    }
+// The way back; returns when the copy has read its source (the bytes land in order for whoever waits for the kernel).
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.commit_group;\n cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
-// Stores the gradients of four neighbouring columns; `vec`: the output row has the input row's alignment.
-__device__ __forceinline__ void store4(float* g, float4 v, bool vec) {
-    if (vec) {
-        __stcs(reinterpret_cast<float4*>(g), v);
-    } else {
-        g[0] = v.x; g[1] = v.y; g[2] = v.z; g[3] = v.w;
-    }
-}
-
-// ---- gradient from saved statistics ----------------------------------------------------------------------
-template <class L, int NV>
-__global__ void __launch_bounds__(kRowThreads)
-row_grad_kernel(const RowParams p, const L loss) {
-    extern __shared__ __align__(16) uint8_t dyn[];
-    const int64_t row = blockIdx.x / p.parts;
-    const int part = blockIdx.x % p.parts;
-    const float* x = p.x + row * p.ncol;
-    float* gx = p.gx + row * p.ncol;
-    const RowShape shape(x, p.ncol, p.parts);
-    const typename L::Smem sm = loss.smem(dyn);
-    const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15) == 0;
-    const float4* xq = reinterpret_cast<const float4*>(x + shape.head);
-    const int64_t q_end = min(shape.quads, (part + 1) * shape.per);
-    const int64_t q_begin = part * shape.per + threadIdx.x;
-    float4 v[NV];
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-        const int64_t q = q_begin + u * kRowThreads;
-        v[u] = (q < q_end) ? __ldcs(xq + q) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    const bool has_loose = part == 0 && static_cast<int>(threadIdx.x) < shape.loose;
-    const float lv = has_loose ? x[shape.loose_col(threadIdx.x)] : 0.0f;
-    loss.gather(sm, nullptr, row, p.ncol);
-    // the labels' logits are read before anything is written: gx may be x
-    const float inv_t = 1.0f / loss.temperature();
-    const float top = p.ps[3 * row], total = p.ps[3 * row + 1], slope = p.ps[3 * row + 2];
-    const float gy = (p.gy != nullptr) ? p.gy[row] : 1.0f;
-    __syncthreads();
-    loss.teacher(sm, p.ncol);
-    __syncthreads();
-    loss.merge(sm);
-    const int state = loss.state(sm);
-    const float k = loss.q_coef(gy, slope);
-    // one factor for all columns; a padding row's logits are not looked at, a bad label poisons the row
-    const float f = k / total;
-    auto grad = [&](float xv) {
-        return state == kLive ? weight(xv, top, inv_t) * f : (state == kPadding ? 0.0f : nanf(""));
-    };
-    // labelled columns of this part: value in registers until the columns around them are written
-    for (int base = 0; base < loss.labels(); base += kRowThreads) {
-        // gathered in rounds of one label per thread; rounds beyond the first only for more than 512 labels
-        const int j = base + threadIdx.x;
-        int64_t c = 0;
-        float w = 0.0f;
-        bool mine = state == kLive && j < loss.labels() && loss.label(sm, j, c, w) && shape.owned(c, part);
-        float g = 0.0f;
-        if (mine) g = weight(x[c], top, inv_t) * f - k * w;
-        __syncthreads();
-        if (mine) sm.xz[j] = g;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-        const int64_t q = q_begin + u * kRowThreads;
-        if (q < q_end)
-            store4(gx + shape.head + 4 * q, make_float4(grad(v[u].x), grad(v[u].y), grad(v[u].z), grad(v[u].w)), vec);
-    }
-    if (has_loose) gx[shape.loose_col(threadIdx.x)] = grad(lv);
-    __syncthreads();
-    for (int j = threadIdx.x; j < loss.labels(); j += kRowThreads) {
-        int64_t c = 0;
-        float w = 0.0f;
-        if (state == kLive && loss.label(sm, j, c, w) && shape.owned(c, part)) gx[c] = sm.xz[j];
-    }
-}
-
-// ---- loss and gradient with one read -----------------------------------------------------------------------
-// The row is spread over the registers of `parts` CTAs (a cluster, 1 to 8), NV 16-byte pieces per thread.  Each CTA
-// forms its maximum and sum of exponentials, the cluster exchanges the two numbers through distributed shared memory,
-// and the gradient is one multiplication per value.
-template <class L, int NV>
-__global__ void __launch_bounds__(kRowThreads)
-row_step_kernel(const RowParams p, const L loss) {
-    extern __shared__ __align__(16) uint8_t dyn[];
-    __shared__ float red_m[kRowWarps], red_s[kRowWarps];
-    __shared__ float2 stat[8];
-    __shared__ float slope_sh;
-    const int64_t row = blockIdx.x / p.parts;
-    const int part = blockIdx.x % p.parts;
-    if (p.parts > 1) cluster_arrive();
-    const float* x = p.x + row * p.ncol;
-    float* gx = p.gx + row * p.ncol;
-    const RowShape shape(x, p.ncol, p.parts);
-    const typename L::Smem sm = loss.smem(dyn);
-    const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15) == 0;
-    const float4* xq = reinterpret_cast<const float4*>(x + shape.head);
-    const int64_t q_end = min(shape.quads, (part + 1) * shape.per);
-    const int64_t q_begin = part * shape.per + threadIdx.x;
-    float4 v[NV];
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-        const int64_t q = q_begin + u * kRowThreads;
-        v[u] = (q < q_end) ? __ldcs(xq + q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    }
-    const bool has_loose = part == 0 && static_cast<int>(threadIdx.x) < shape.loose;
-    float lv = has_loose ? x[shape.loose_col(threadIdx.x)] : -INFINITY;
-    loss.gather(sm, x, row, p.ncol);
-    const float inv_t = 1.0f / loss.temperature();
-    const float gy = (p.gy != nullptr) ? p.gy[row] : 1.0f;
-
-    float m = lv;
-#pragma unroll
-    for (int u = 0; u < NV; ++u) max4(v[u], m);
-    const float mine_top = block_max(m, red_m);
-    loss.teacher(sm, p.ncol);
+// Joins `n` pairs (reference, sum of exponentials against it); every warp does the same in the same order.
+__device__ __forceinline__ void join(const float2* stat, int n, float& k, float& total) {
+    const int lane = threadIdx.x & 31;
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, stat[i].x);
+    k = warp_max(m);
+    const float kf = finite_ref(k);
     float s = 0.0f;
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-        v[u] = make_float4(weight(v[u].x, mine_top, inv_t), weight(v[u].y, mine_top, inv_t),
-                           weight(v[u].z, mine_top, inv_t), weight(v[u].w, mine_top, inv_t));
-        s += (v[u].x + v[u].y) + (v[u].z + v[u].w);
+    for (int i = lane; i < n; i += 32) s += stat[i].y * exp2_approx(stat[i].x - kf);
+    total = warp_sum(s);
+}
+
+// Losses and statistics of `n` parked rows first, first + step, ...: a lane each.
+template <class L>
+__device__ __forceinline__ void settle_rows(const RowParams& p, const L& loss, const typename L::Parked* q, int n, int64_t first,
+                                            int64_t step, const Temp& tv) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    if (lane < n) {
+        const int64_t row = first + lane * step;
+        Result res = loss.settle(q, lane, tv);
+        const int state = q->state[lane];
+        if (state == kPadding) res.loss = res.slope = res.logp = 0.0f;
+        if (state == kBad) res.loss = res.slope = res.logp = nanf("");
+        p.y[row] = res.loss;
+        loss.extra(row, res.logp);
+        if (p.ps != nullptr) {
+            p.ps[3 * row + 0] = q->k[lane];
+            p.ps[3 * row + 1] = q->total[lane];
+            p.ps[3 * row + 2] = res.slope;
+        }
+        if (state == kBad) *p.flag = 1;
     }
-    if (has_loose) { lv = weight(lv, mine_top, inv_t); s += lv; }
-    float top = mine_top, total = block_sum(s, red_s);
-    if (p.parts > 1) {
-        cluster_wait();                         // every CTA of the cluster has begun
-        if (static_cast<int>(threadIdx.x) < p.parts) push_stat(&stat[part], threadIdx.x, top, total);
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();                         // all labels are gathered and all statistics here: x may be written
-        join(stat, p.parts, inv_t, top, total);
+    __syncwarp();
+}
+
+template <class L, int T, int MODE>
+__global__ void __launch_bounds__(T + 32, T == 64 ? 10 : T == 128 ? 6 : 1)
+row_stream_kernel(const RowParams p, const L loss) {
+    constexpr int W = T / 32;
+    extern __shared__ __align__(16) uint8_t dyn[];
+    __shared__ float2 stat[2][kMaxParts * W];
+    __shared__ float loose_sh[8];
+    __shared__ uint64_t full;
+    __shared__ int abort_flag;
+    using Row = typename L::Row;
+    float4* stage = reinterpret_cast<float4*>(dyn);                      // this part of the row
+    uint8_t* rows = dyn + p.per * sizeof(float4);                        // [2] label buffers
+    const size_t row_bytes = loss.bytes();
+    typename L::Parked* parked = reinterpret_cast<typename L::Parked*>(rows + 2 * row_bytes);
+    const int ncol = static_cast<int>(p.ncol);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+    const bool labels = warp == W;                                       // the warp that prepares labels
+    const int part = blockIdx.x % p.parts;
+    const int64_t first = blockIdx.x / p.parts, step = gridDim.x / p.parts;
+    const Temp tv(p.temp);
+    const bool cluster = MODE != kGrad && p.parts > 1;
+    if (tid == 0) {
+        mbar_init(smem_u32(&full), 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    const int state = loss.state(sm);
-    if (threadIdx.x < 32) {
-        RowResult r = loss.finish(sm, top, total, row);
-        if (state == kPadding) r.loss = r.slope = r.logp = 0.0f;
-        if (state == kBad) r.loss = r.slope = r.logp = nanf("");
-        if (threadIdx.x == 0) {
-            slope_sh = r.slope;
-            if (part == 0) {
-                p.y[row] = r.loss;
-                loss.extra(row, r.logp);
-                if (state == kBad) *p.flag = 1;
+    if (cluster) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
+
+    auto fetch = [&](int64_t row) {
+        const float* x = p.x + row * p.ncol;
+        const RowShape shape(x, ncol, p.per);
+        const uint32_t bytes = static_cast<uint32_t>(shape.count(part)) * 16u;
+        mbar_expect_tx(smem_u32(&full), bytes);
+        if (bytes > 0)
+            bulk_load(stage, reinterpret_cast<const float4*>(x + shape.head) + shape.begin(part), bytes, smem_u32(&full));
+    };
+
+    // The label warp's three stages; every part of a row needs all labels' logits (kStep: the policy's slope hangs on them)
+    // or its own (kGrad).
+    typename L::Ahead ids, ids_next;
+    typename L::Flight flight;
+    float gy_next = 1.0f, ps_next = 0.0f;
+    auto depart = [&](int64_t row) {
+        const float* x = p.x + row * p.ncol;
+        const RowShape shape(x, ncol, p.per);
+        loss.depart(flight, ids, x, shape, part, MODE != kGrad, row, p.ncol);
+        if (MODE != kLoss && p.gy != nullptr) gy_next = p.gy[row];
+        if (MODE == kGrad && lane < 3) ps_next = p.ps[3 * row + lane];
+    };
+    auto arrive = [&](int64_t row, int buf) {
+        const float* x = p.x + row * p.ncol;
+        const RowShape shape(x, ncol, p.per);
+        Row* r = reinterpret_cast<Row*>(rows + buf * row_bytes);
+        if (lane == 0) r->gy = gy_next;
+        if (MODE == kGrad && lane < 3) r->stat[lane] = ps_next;
+        loss.arrive(r, flight, ids, x, shape, part, MODE != kGrad, row, p.ncol, tv);
+    };
+
+    if (first < p.nrow) {
+        if (labels) {
+            loss.ahead(ids, first);
+            depart(first);
+            arrive(first, 0);
+            if (first + step < p.nrow) loss.ahead(ids, first + step);
+        } else if (tid == 0) {
+            fetch(first);
+        }
+    }
+
+    int buf = 0, waiting = 0;
+    uint32_t phase = 0;
+    for (int64_t row = first; row < p.nrow; row += step, buf ^= 1, phase ^= 1u) {
+        const int64_t next = row + step;
+        Row* r = reinterpret_cast<Row*>(rows + buf * row_bytes);
+        const float* x = p.x + row * p.ncol;
+        const RowShape shape(x, ncol, p.per);
+        const int n = shape.count(part);           // 16-byte pieces of this part
+        const bool loose = part == 0 && tid < shape.loose;
+        float lv = -INFINITY;
+        if (!labels) {
+            if (loose) lv = x[shape.loose_col(tid)];
+            mbar_wait(smem_u32(&full), phase, &abort_flag, p.status, 40);
+            if (MODE != kGrad) {
+                float m = lv;
+#pragma unroll 4
+                for (int i = tid; i < n; i += T) m = max4(stage[i], m);
+                const float k = reference(warp_max(m), tv.c);
+                const float kf = finite_ref(k);
+                float s = weight(lv, kf, tv.c);
+#pragma unroll 4
+                for (int i = tid; i < n; i += T) s += weight4(stage[i], kf, tv.c);
+                s = warp_sum(s);
+                if (cluster) {
+                    if (lane < p.parts) push_stat(&stat[buf][part * W + warp], lane, k, s);
+                } else if (lane == 0) {
+                    stat[buf][warp] = make_float2(k, s);
+                }
+                __syncwarp();
+            }
+        }
+        // The one barrier of all parts: the row's statistics and labels are there, and the labels' logits have been read
+        // everywhere, so that the gradient may be written over them.  The list of statistics and the label buffer are used
+        // in turn: a CTA that fills one again has passed the next row's barrier, where everybody is done with it.
+        if (cluster) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
+
+        if (labels) {
+            if (next < p.nrow) {
+                depart(next);
+                if (next + step < p.nrow) loss.ahead(ids_next, next + step);
+            }
+            if (MODE != kGrad && part == 0) {
+                float k, total;
+                join(stat[buf], p.parts * W, k, total);
+                loss.park(parked, waiting, r, k, total, tv);
+                if (++waiting == kParked || next >= p.nrow) {
+                    settle_rows(p, loss, parked, waiting, row - (waiting - 1) * step, step, tv);
+                    waiting = 0;
+                }
+            } else if (MODE == kGrad && part == 0 && lane == 0 && r->state == kBad) {
+                *p.flag = 1;
+            }
+            if (next < p.nrow) {
+                arrive(next, buf ^ 1);
+                ids = ids_next;
+            }
+        } else if (MODE == kLoss) {
+            if (tid == 0 && next < p.nrow) fetch(next);
+        } else {
+            float k, total, slope;
+            if (MODE == kGrad) {
+                k = r->stat[0]; total = r->stat[1]; slope = r->stat[2];
+            } else {
+                join(stat[buf], p.parts * W, k, total);
+                slope = loss.finish_slope(r, k, total, tv);
+            }
+            const float kf = finite_ref(k);
+            const float coef = loss.coef(r, slope, tv);
+            const float f = coef / total;                                   // gradient = f * 2^(x c - k)
+            const int state = r->state;
+            float* gx = p.gx + row * p.ncol;
+            if (state == kLive) {
+#pragma unroll 4
+                for (int i = tid; i < n; i += T) {
+                    const float4 v = stage[i];
+                    stage[i] = make_float4(weight(v.x, kf, tv.c) * f, weight(v.y, kf, tv.c) * f, weight(v.z, kf, tv.c) * f,
+                                           weight(v.w, kf, tv.c) * f);
+                }
+                if (loose) loose_sh[tid] = weight(lv, kf, tv.c) * f;
+                asm volatile("bar.sync 1, %0;" ::"n"(T) : "memory");
+                // the labels' columns, over what has just been written there
+                const int g = loss.sharers(T);
+                for (int j0 = 0; j0 < loss.labels(); j0 += T / g) {
+                    const int j = j0 + tid / g;
+                    int c;
+                    float w, xv;
+                    if (loss.label(r, j, tid % g, g, c, w, xv) && shape.owned(c, part)) {
+                        const float v = weight(xv, kf, tv.c) * f - coef * w;
+                        const int q = (c - shape.head) >> 2;
+                        if (c < shape.head) loose_sh[c] = v;
+                        else if (q >= shape.quads) loose_sh[c - 4 * shape.quads] = v;
+                        else reinterpret_cast<float*>(stage)[c - shape.head - 4 * shape.begin(part)] = v;
+                    }
+                }
+            } else {
+                // a padding row's logits are not looked at; a bad label poisons the row
+                const float fixed = state == kPadding ? 0.0f : nanf("");
+                for (int i = tid; i < n; i += T) stage[i] = make_float4(fixed, fixed, fixed, fixed);
+                if (loose) loose_sh[tid] = fixed;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the bulk copy reads what this thread wrote
+            asm volatile("bar.sync 1, %0;" ::"n"(T) : "memory");
+            if (loose) gx[shape.loose_col(tid)] = loose_sh[tid];
+            float* out = gx + shape.head + 4 * shape.begin(part);
+            if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15) == 0) {
+                if (tid == 0) {
+                    if (n > 0) bulk_store(out, stage, static_cast<uint32_t>(n) * 16u);
+                    if (next < p.nrow) fetch(next);
+                }
+            } else {
+                // the gradient's rows lie on another 4-byte phase than the logits'
+                for (int i = tid; i < 4 * n; i += T) out[i] = reinterpret_cast<const float*>(stage)[i];
+                asm volatile("bar.sync 1, %0;" ::"n"(T) : "memory");
+                if (tid == 0 && next < p.nrow) fetch(next);
             }
         }
     }
     __syncthreads();
-    loss.merge(sm);
-    const float k = loss.q_coef(gy, slope_sh);
-    const float f = k / total;
-    const float f_mine = f * weight(mine_top, top, inv_t);
-    auto grad = [&](float e) { return state == kLive ? e * f_mine : (state == kPadding ? 0.0f : nanf("")); };
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-        const int64_t q = q_begin + u * kRowThreads;
-        if (q < q_end)
-            store4(gx + shape.head + 4 * q, make_float4(grad(v[u].x), grad(v[u].y), grad(v[u].z), grad(v[u].w)), vec);
+    if (abort_flag) {          // copies may still be on their way into this CTA's memory
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
     }
-    if (has_loose) gx[shape.loose_col(threadIdx.x)] = grad(lv);
-    __syncthreads();
-    for (int j = threadIdx.x; j < loss.labels(); j += kRowThreads) {
-        int64_t c = 0;
-        float w = 0.0f;
-        if (state == kLive && loss.label(sm, j, c, w) && shape.owned(c, part))
-            gx[c] = weight(sm.xz[j], top, inv_t) * f - k * w;
+}
+
+// ---- rows of any length, loss and statistics alone -------------------------------------------------------
+// A thread keeps a running reference k and sum s over its pieces of the row, four 16-byte loads at a time: the maximum of
+// the sixteen values first, one rescaling of s (a power of two) if it rose, then sixteen exponentials.
+template <class L>
+__global__ void __launch_bounds__(512 + 32)
+row_loss_wide_kernel(const RowParams p, const L loss) {
+    constexpr int T = 512, W = T / 32;
+    extern __shared__ __align__(16) uint8_t dyn[];
+    __shared__ float2 stat[kMaxParts * W];
+    const int64_t row = blockIdx.x / p.parts;
+    const int part = blockIdx.x % p.parts;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Temp tv(p.temp);
+    const int ncol = static_cast<int>(p.ncol);
+    const float* x = p.x + row * p.ncol;
+    const RowShape shape(x, ncol, p.per);
+    typename L::Row* r = reinterpret_cast<typename L::Row*>(dyn);
+    if (p.parts > 1) { cluster_arrive(); cluster_wait(); }
+    if (warp == W) {
+        if (part == 0) {
+            typename L::Ahead ids;
+            typename L::Flight flight;
+            loss.ahead(ids, row);
+            loss.depart(flight, ids, x, shape, part, true, row, p.ncol);
+            loss.arrive(r, flight, ids, x, shape, part, true, row, p.ncol, tv);
+        }
+    } else {
+        const float4* xq = reinterpret_cast<const float4*>(x + shape.head);
+        const int q_end = shape.begin(part) + shape.count(part);
+        float k = -INFINITY, s = 0.0f;
+        if (part == 0 && static_cast<int>(threadIdx.x) < shape.loose) {
+            const float v = x[shape.loose_col(threadIdx.x)];
+            k = reference(v, tv.c);
+            s = weight(v, finite_ref(k), tv.c);
+        }
+        for (int q0 = shape.begin(part) + threadIdx.x; q0 < q_end; q0 += 4 * T) {
+            float4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                v[u] = (q0 + u * T < q_end) ? __ldcs(xq + q0 + u * T)
+                                            : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            float m = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) m = max4(v[u], m);
+            const float k1 = reference(m, tv.c);
+            if (k1 > k) { s *= exp2_approx(k - k1); k = k1; }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s += weight4(v[u], finite_ref(k), tv.c);
+        }
+        const float kw = warp_max(k);
+        s = warp_sum(s * exp2_approx(k - finite_ref(kw)));
+        if (p.parts > 1) {
+            if (lane == 0) push_stat(&stat[part * W + warp], 0, kw, s);
+        } else if (lane == 0) {
+            stat[warp] = make_float2(kw, s);
+        }
+        __syncwarp();
+    }
+    if (p.parts > 1) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
+    if (warp == W && part == 0) {
+        float k, total;
+        join(stat, p.parts * W, k, total);
+        __shared__ typename L::Parked parked;
+        loss.park(&parked, 0, r, k, total, tv);
+        settle_rows(p, loss, &parked, 1, row, 1, tv);
     }
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------
-template <class K, class L>
-int launch_rows(K kernel, const char* name, const RowParams& p, const L& loss, int64_t nrow, bool cluster, size_t smem,
-                cudaStream_t s) {
-    if (nrow * p.parts >= (int64_t(1) << 31)) return fail(KAI_E_TOO_LARGE, "%s: too many rows for one launch", name);
+constexpr int64_t kPart = 8192;       // columns of a part: 32 KB, five or six parts to an SM
+constexpr size_t kSmemMost = 220 * 1024;
+
+// Clusters (or, for `parts` = 1, CTAs) of a kernel that are resident on the device at once: the size of a persistent grid.
+// Asked once per kernel, cluster size and shared-memory size.
+int resident_clusters(const void* kernel, int threads, int parts, size_t smem, int sm_count, int* out) {
+    struct Known { const void* kernel; int device, parts; size_t smem; int clusters; };
+    static std::mutex mu;
+    static std::vector<Known> known;
+    int device = 0;
+    KAI_CUDA(cudaGetDevice(&device));
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        for (const Known& k : known)
+            if (k.kernel == kernel && k.device == device && k.parts == parts && k.smem == smem) { *out = k.clusters; return KAI_OK; }
+    }
+    KAI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMost)));
+    int clusters = 0;
+    if (parts == 1) {
+        int per_sm = 0;
+        KAI_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+        clusters = per_sm * sm_count;
+    } else {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(parts));
+        cfg.blockDim = dim3(static_cast<unsigned>(threads));
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = static_cast<unsigned>(parts);
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        KAI_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg));
+    }
+    if (clusters < 1) return fail(KAI_E_TOO_LARGE, "row losses: %zu bytes of shared memory do not fit", smem);
+    *out = clusters;
+    std::lock_guard<std::mutex> lock(mu);
+    known.push_back(Known{kernel, device, parts, smem, clusters});
+    return KAI_OK;
+}
+
+template <class L>
+int launch_rows(void (*kernel)(const RowParams, const L), const char* name, const RowParams& p, const L& loss, int64_t groups,
+                int threads, bool cluster, size_t smem, cudaStream_t s) {
+    if (groups * p.parts >= (int64_t(1) << 31)) return fail(KAI_E_TOO_LARGE, "%s: too many rows for one launch", name);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(nrow * p.parts));
-    cfg.blockDim = dim3(kRowThreads);
+    cfg.gridDim = dim3(static_cast<unsigned>(groups * p.parts));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -583,113 +802,127 @@ int launch_rows(K kernel, const char* name, const RowParams& p, const L& loss, i
     return KAI_OK;
 }
 
-// CTAs per row of a call that may use up to `most`: as few as hold the row (`need`), and more while the rows alone do not
-// fill the SMs twice and every thread still has a piece.
-int parts_for(int64_t nrow, int64_t ncol, int need, int most, int sm_count) {
-    int parts = need;
-    while (parts * 2 <= most && nrow * parts < 2 * static_cast<int64_t>(sm_count) &&
-           ncol >= static_cast<int64_t>(parts) * 2 * 4 * kRowThreads)
-        parts *= 2;
-    return parts;
+template <class L, int MODE>
+size_t stream_smem(int64_t ncol, int parts, const L& loss) {
+    return ((ncol >> 2) + parts - 1) / parts * sizeof(float4) + 2 * loss.bytes() + (MODE == kGrad ? 0 : sizeof(typename L::Parked));
+}
+
+template <class L, int T, int MODE>
+int launch_stream(DeviceState* st, const RowParams& p0, const L& loss, cudaStream_t s) {
+    RowParams p = p0;
+    auto kernel = row_stream_kernel<L, T, MODE>;
+    p.status = st->status_dev;
+    p.per = static_cast<int>(((p.ncol >> 2) + p.parts - 1) / p.parts);
+    const size_t smem = stream_smem<L, MODE>(p.ncol, p.parts, loss);
+    int clusters = 0;
+    const int group = MODE == kGrad ? 1 : p.parts;
+    KAI_TRY(resident_clusters(reinterpret_cast<const void*>(kernel), T + 32, group, smem, st->sm_count, &clusters));
+    if (MODE == kGrad) clusters = clusters / p.parts < 1 ? 1 : clusters / p.parts;
+    const int64_t groups = p.nrow < clusters ? p.nrow : clusters;
+    return launch_rows(kernel, "row_stream_kernel", p, loss, groups, T + 32, MODE != kGrad, smem, s);
 }
 
 template <class L>
-int run_loss(DeviceState* st, RowParams p, const L& loss, int64_t nrow, size_t smem, cudaStream_t s) {
+int run_wide(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
+    p.parts = kMaxParts;
+    p.per = static_cast<int>(((p.ncol >> 2) + kMaxParts - 1) / kMaxParts);
+    (void)st;
+    return launch_rows(row_loss_wide_kernel<L>, "row_loss_wide_kernel", p, loss, p.nrow, 512 + 32, true, loss.bytes(), s);
+}
+
+// Parts of a row: as many as hold it at kPart columns, and more while the rows alone do not fill the SMs and a part keeps 1024
+// columns.
+int row_parts(int64_t nrow, int64_t ncol, int64_t most, int sm_count) {
+    int64_t parts = 1;
+    while (parts < most && parts * kPart < ncol) parts *= 2;
+    while (parts * 2 <= most && nrow * parts < 2 * static_cast<int64_t>(sm_count) && ncol >= parts * 2 * 1024) parts *= 2;
+    return static_cast<int>(parts);
+}
+
+// Threads of a CTA: 64 for many short rows (a part of 2048 columns at most), 256 for parts beyond kPart and where there are too few
+// parts to give every SM four, 128 otherwise.
+template <class L, int MODE>
+int launch_threads(DeviceState* st, const RowParams& p, const L& loss, cudaStream_t s) {
+    const int64_t each = (p.ncol + p.parts - 1) / p.parts, ctas = p.nrow * p.parts;
+    if (each > kPart || ctas < 4 * static_cast<int64_t>(st->sm_count)) return launch_stream<L, 256, MODE>(st, p, loss, s);
+    if (each <= 2048) return launch_stream<L, 64, MODE>(st, p, loss, s);
+    return launch_stream<L, 128, MODE>(st, p, loss, s);
+}
+
+template <class L>
+int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
-    p.parts = parts_for(nrow, p.ncol, 1, 8, st->sm_count);
-    return launch_rows(row_loss_kernel<L>, "row_loss_kernel", p, loss, nrow, true, smem, s);
+    p.parts = row_parts(p.nrow, p.ncol, int64_t(1) << 20, st->sm_count);
+    return launch_threads<L, kGrad>(st, p, loss, s);
 }
 
-template <class L>
-int run_grad(DeviceState* st, RowParams p, const L& loss, int64_t nrow, size_t smem, cudaStream_t s) {
+template <class L, int MODE>
+int run_rows(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
-    const int64_t per = 4 * kRowThreads;
-    const int64_t pieces = (p.ncol + per - 1) / per;       // 16-byte pieces per thread over the whole row
-    int64_t parts = (pieces + 7) / 8;
-    if (parts < 1) parts = 1;
-    const int64_t each = (pieces + parts - 1) / parts;
-    p.parts = static_cast<int>(parts);
-    if (each <= 1) return launch_rows(row_grad_kernel<L, 1>, "row_grad_kernel", p, loss, nrow, false, smem, s);
-    if (each <= 2) return launch_rows(row_grad_kernel<L, 2>, "row_grad_kernel", p, loss, nrow, false, smem, s);
-    if (each <= 4) return launch_rows(row_grad_kernel<L, 4>, "row_grad_kernel", p, loss, nrow, false, smem, s);
-    return launch_rows(row_grad_kernel<L, 8>, "row_grad_kernel", p, loss, nrow, false, smem, s);
-}
-
-template <class L>
-int run_step(DeviceState* st, RowParams p, const L& loss, int64_t nrow, size_t smem, cudaStream_t s) {
-    const int64_t cap = 8 * 4 * kRowThreads;        // values a CTA holds at 8 pieces per thread
-    int need = 1;
-    while (need < 8 && need * cap < p.ncol) need *= 2;
-    if (need * cap < p.ncol) {                      // a row that a cluster cannot hold: two kernels, two reads
-        KAI_TRY(ensure_aux(st, nrow * 3 * 4));
+    if (stream_smem<L, MODE>(p.ncol, kMaxParts, loss) > kSmemMost) {
+        if (MODE == kLoss) return run_wide(st, p, loss, s);
+        KAI_TRY(ensure_aux(st, p.nrow * 3 * 4));
         p.ps = static_cast<float*>(st->aux);
-        KAI_TRY(run_loss(st, p, loss, nrow, smem, s));
-        return run_grad(st, p, loss, nrow, smem, s);
+        KAI_TRY(run_wide(st, p, loss, s));
+        return run_grad(st, p, loss, s);
     }
-    p.flag = st->flag_dev + 2;
-    p.parts = parts_for(nrow, p.ncol, need, 8, st->sm_count);
-    const int64_t per = static_cast<int64_t>(p.parts) * 4 * kRowThreads;
-    const int64_t each = (p.ncol + per - 1) / per;
-    if (each <= 1) return launch_rows(row_step_kernel<L, 1>, "row_step_kernel", p, loss, nrow, true, smem, s);
-    if (each <= 2) return launch_rows(row_step_kernel<L, 2>, "row_step_kernel", p, loss, nrow, true, smem, s);
-    if (each <= 4) return launch_rows(row_step_kernel<L, 4>, "row_step_kernel", p, loss, nrow, true, smem, s);
-    return launch_rows(row_step_kernel<L, 8>, "row_step_kernel", p, loss, nrow, true, smem, s);
+    p.parts = row_parts(p.nrow, p.ncol, kMaxParts, st->sm_count);
+    return launch_threads<L, MODE>(st, p, loss, s);
 }
 
-RowParams row_params(const float* x, int64_t ncol) {
+RowParams row_params(const float* x, int64_t nrow, int64_t ncol, const float* temp) {
     RowParams p{};
     p.x = x;
+    p.nrow = nrow;
     p.ncol = ncol;
+    p.temp = temp;
     p.parts = 1;
     return p;
+}
+Distill distill(const int* idx, const float* t, int64_t ntop) {
+    return Distill{idx, t, static_cast<int>(ntop), static_cast<int>((ntop + 3) / 4 * 4)};
 }
 
 }  // namespace
 
 int loss_distill(DeviceState* st, float* y, float* ps, const float* x, const int* idx, const float* t, int64_t nrow,
                  int64_t ncol, int64_t ntop, const float* temp, cudaStream_t s) {
-    RowParams p = row_params(x, ncol);
+    RowParams p = row_params(x, nrow, ncol, temp);
     p.y = y; p.ps = ps;
-    const Distill d{idx, t, temp, static_cast<int>(ntop)};
-    return run_loss(st, p, d, nrow, Distill::smem_bytes(d.ntop), s);
+    return run_rows<Distill, kLoss>(st, p, distill(idx, t, ntop), s);
 }
 int loss_distill_backward(DeviceState* st, float* gx, const float* gy, const float* x, const float* ps, const int* idx,
                           const float* t, int64_t nrow, int64_t ncol, int64_t ntop, const float* temp, cudaStream_t s) {
-    RowParams p = row_params(x, ncol);
+    RowParams p = row_params(x, nrow, ncol, temp);
     p.gx = gx; p.gy = gy; p.ps = const_cast<float*>(ps);
-    const Distill d{idx, t, temp, static_cast<int>(ntop)};
-    return run_grad(st, p, d, nrow, Distill::smem_bytes(d.ntop), s);
+    return run_grad(st, p, distill(idx, t, ntop), s);
 }
 int loss_distill_step(DeviceState* st, float* y, float* gx, const float* gy, const float* x, const int* idx,
                       const float* t, int64_t nrow, int64_t ncol, int64_t ntop, const float* temp, cudaStream_t s) {
-    RowParams p = row_params(x, ncol);
+    RowParams p = row_params(x, nrow, ncol, temp);
     p.y = y; p.gx = gx; p.gy = gy;
-    const Distill d{idx, t, temp, static_cast<int>(ntop)};
-    return run_step(st, p, d, nrow, Distill::smem_bytes(d.ntop), s);
+    return run_rows<Distill, kStep>(st, p, distill(idx, t, ntop), s);
 }
 
 int loss_policy(DeviceState* st, float* y, float* logp, float* ps, const float* x, const int* z, const float* old_logp,
                 const float* ref_logp, const float* adv, int64_t nrow, int64_t ncol, const float* low, const float* high,
                 const float* beta, const float* temp, cudaStream_t s) {
-    RowParams p = row_params(x, ncol);
+    RowParams p = row_params(x, nrow, ncol, temp);
     p.y = y; p.ps = ps;
-    const Policy l{z, old_logp, ref_logp, adv, low, high, beta, temp, logp};
-    return run_loss(st, p, l, nrow, Policy::smem_bytes(1), s);
+    return run_rows<Policy, kLoss>(st, p, Policy{z, old_logp, ref_logp, adv, low, high, beta, logp}, s);
 }
 int loss_policy_backward(DeviceState* st, float* gx, const float* gy, const float* x, const float* ps, const int* z,
                          int64_t nrow, int64_t ncol, const float* temp, cudaStream_t s) {
-    RowParams p = row_params(x, ncol);
+    RowParams p = row_params(x, nrow, ncol, temp);
     p.gx = gx; p.gy = gy; p.ps = const_cast<float*>(ps);
-    const Policy l{z, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, temp, nullptr};
-    return run_grad(st, p, l, nrow, Policy::smem_bytes(1), s);
+    return run_grad(st, p, Policy{z, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr}, s);
 }
 int loss_policy_step(DeviceState* st, float* y, float* logp, float* gx, const float* gy, const float* x, const int* z,
                      const float* old_logp, const float* ref_logp, const float* adv, int64_t nrow, int64_t ncol,
                      const float* low, const float* high, const float* beta, const float* temp, cudaStream_t s) {
-    RowParams p = row_params(x, ncol);
+    RowParams p = row_params(x, nrow, ncol, temp);
     p.y = y; p.gx = gx; p.gy = gy;
-    const Policy l{z, old_logp, ref_logp, adv, low, high, beta, temp, logp};
-    return run_step(st, p, l, nrow, Policy::smem_bytes(1), s);
+    return run_rows<Policy, kStep>(st, p, Policy{z, old_logp, ref_logp, adv, low, high, beta, logp}, s);
 }
 
 }  // namespace kai

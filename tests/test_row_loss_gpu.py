@@ -86,7 +86,8 @@ def _near(got, want, tol):
 
 
 SHAPES = [(1, 1, 1), (1, 2, 5), (3, 5, 5), (7, 33, 4), (2, 1000, 64), (5, 2047, 3), (3, 4099, 600), (1, 32000, 32),
-          (2, 50257, 64), (300, 130, 8), (2, 128256, 17), (1, 131073, 9), (2, 140001, 40), (600, 2100, 1), (2, 300, 2048)]
+          (2, 50257, 64), (300, 130, 8), (2, 128256, 17), (1, 131073, 9), (2, 140001, 40), (600, 2100, 1), (2, 300, 2048), (2, 380001, 1500),
+          (1, 450001, 30), (700, 1030, 5)]
 
 
 @pytest.mark.parametrize("mode", ["step", "calls"])
@@ -133,7 +134,7 @@ def test_distill_alignments_repeats_and_gaps(torch_cuda, vm, off, mode):
 
 
 @pytest.mark.parametrize("mode", ["step", "calls"])
-@pytest.mark.parametrize("ncol", [40, 9000, 140001])
+@pytest.mark.parametrize("ncol", [40, 9000, 440001])
 def test_distill_infinities(torch_cuda, vm, mode, ncol):
     """Logits of -inf (a masked vocabulary) have no probability; the type's lowest value behaves as such; a labelled -inf is an infinite
     loss; NaN and +inf poison their own row only."""
@@ -239,7 +240,7 @@ def _policy_inputs(n, c, temp, seed):
 
 
 @pytest.mark.parametrize("mode", ["step", "calls"])
-@pytest.mark.parametrize("shape", [(1, 1), (9, 2), (40, 37), (3, 4097), (5, 32000), (2, 50257), (2, 128256), (1, 200003),
+@pytest.mark.parametrize("shape", [(1, 1), (9, 2), (40, 37), (3, 4097), (5, 32000), (2, 50257), (2, 128256), (1, 200003), (1, 460003),
                                    (700, 500)])
 def test_policy(torch_cuda, vm, shape, mode):
     n, c = shape
@@ -296,7 +297,7 @@ def test_policy_gradient_against_differences(torch_cuda, vm):
 
 
 # ---- both ----------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("ncol", [7, 50257, 140001])
+@pytest.mark.parametrize("ncol", [7, 50257, 440001])
 def test_gradient_over_the_logits_and_default_gradient(torch_cuda, vm, ncol):
     """pgx = px, and pgy = NULL: the same bits as with buffers of their own and a gradient of ones."""
     torch = torch_cuda
