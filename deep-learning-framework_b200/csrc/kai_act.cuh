@@ -77,6 +77,12 @@ __device__ __forceinline__ float act_grad_from_x(int act, float x, float leaky_a
     }
 }
 
+// Value and slope of one pre-activation, as a call: a kernel that evaluates many per thread would otherwise hold a copy of all
+// cases for each and spend its time fetching instructions.
+static __device__ __noinline__ float2 act_value_slope(int act, float x, float leaky_alpha) {
+    return make_float2(act_forward(act, x, leaky_alpha), act_grad_from_x(act, x, leaky_alpha));
+}
+
 // d act / d x evaluated on the OUTPUT y (vmath.cu:3411-3444); only these five exist there.
 __device__ __forceinline__ float act_grad_from_y(int act, float y, float leaky_alpha) {
     switch (act) {

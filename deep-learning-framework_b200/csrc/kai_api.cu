@@ -52,8 +52,15 @@ int ew_layernorm_backward(float*, const float*, const float*, int64_t, int64_t, 
 int rotary(DeviceState*, float*, const float*, const double*, const int64_t*, int64_t, int64_t, int64_t, int64_t, int64_t,
            int64_t, int, const float*, int64_t, int64_t, int, cudaStream_t);
 int rotary_frequencies(double*, int64_t, double, int, double, double, double, int64_t, cudaStream_t);
-int gated_apply(DeviceState*, float*, float*, float*, const float*, const float*, int64_t, int64_t, int, const float*, int,
-                cudaStream_t);
+int gated_forward_tc(DeviceState*, int, float*, float*, float*, const float*, const float*, const float*, const float*,
+                     const float*, int64_t, int64_t, int64_t, int, const float*, cudaStream_t);
+int gated_backward_tc(DeviceState*, int, float*, float*, float*, float*, float*, const float*, const float*, const float*,
+                      const float*, const float*, const float*, int64_t, int64_t, int64_t, int, const float*, int, int,
+                      cudaStream_t);
+int gated_forward_mma(DeviceState*, float*, float*, float*, const float*, const float*, const float*, const float*, const float*,
+                      int64_t, int64_t, int64_t, int, const float*, cudaStream_t);
+int gated_backward_mma(DeviceState*, float*, float*, float*, const float*, const float*, const float*, const float*,
+                       const float*, int64_t, int64_t, int64_t, int, int, cudaStream_t);
 int gated_apply_backward(DeviceState*, float*, float*, const float*, const float*, const float*, int64_t, int,
                          const float*, cudaStream_t);
 int loss_distill(DeviceState*, float*, float*, const float*, const int*, const float*, int64_t, int64_t, int64_t,
@@ -481,6 +488,9 @@ int kai_set_option(const char* name, int64_t value) {
     } else if (!strcmp(name, "tc_min_flops")) {
         if (value < 0) return fail(KAI_E_INVALID_ARG, "tc_min_flops must be >= 0");
         o.tc_min_flops = value;
+    } else if (!strcmp(name, "gated_tc_flops")) {
+        if (value < 0) return fail(KAI_E_INVALID_ARG, "gated_tc_flops must be >= 0");
+        o.gated_tc_flops = value;
     } else if (!strcmp(name, "split_k")) {
         if (value < 0 || value > 64) return fail(KAI_E_INVALID_ARG, "split_k must be in 0..64");
         o.split_k = value;
@@ -545,6 +555,7 @@ int64_t kai_get_option(const char* name) {
     if (!strcmp(name, "tc_bn")) return o.tc_bn;
     if (!strcmp(name, "tc_bk")) return o.tc_bk;
     if (!strcmp(name, "tc_min_flops")) return o.tc_min_flops;
+    if (!strcmp(name, "gated_tc_flops")) return o.gated_tc_flops;
     if (!strcmp(name, "split_k")) return o.split_k;
     if (!strcmp(name, "path")) return o.path;
     if (!strcmp(name, "tc_group_m")) return o.tc_group_m;
@@ -1465,17 +1476,10 @@ int kai_gated_linear_forward(int device, float* ph, float* pg, float* pu, const 
         return fail(KAI_E_INVALID_ARG, "gated_linear_forward: an output overlaps another output or px");
     KAI_ENTER(device);
     if (ndat == 0 || yvec == 0) return KAI_OK;
-    const int save = pg != nullptr;
-    if (!save) {
-        KAI_TRY(ensure_aux(st, 2 * ndat * yvec * 4));
-        pg = static_cast<float*>(st->aux);
-        pu = pg + ndat * yvec;
-    }
-    KAI_TRY(kai_sgemm(device, KAI_GEMM_NT, pg, px, pwg, ndat, yvec, xvec, yvec, 0, nullptr, KAI_ACT_NONE, nullptr,
-                      KAI_PATH_AUTO, stream));
-    KAI_TRY(kai_sgemm(device, KAI_GEMM_NT, pu, px, pwu, ndat, yvec, xvec, yvec, 0, nullptr, KAI_ACT_NONE, nullptr,
-                      KAI_PATH_AUTO, stream));
-    return gated_apply(st, ph, pg, pu, pbg, pbu, ndat, yvec, act, leaky_alpha, save, s);
+    const double flops = 4.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
+    if (xvec > 0 && ndat > 16 && flops >= static_cast<double>(options().gated_tc_flops.load()))
+        return gated_forward_tc(st, device, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
+    return gated_forward_mma(st, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
 }
 
 int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float* pgwu, float* pgg, float* pgu, const float* pgh,
@@ -1501,21 +1505,16 @@ int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float* pgwu, 
     }
     if (clash) return fail(KAI_E_INVALID_ARG, "gated_linear_backward: two buffers overlap");
     KAI_ENTER(device);
+    const double flops = 8.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
+    if (ndat > 16 && flops > 0.0 && flops >= static_cast<double>(options().gated_tc_flops.load()) && (pgx || pgwg))
+        return gated_backward_tc(st, device, pgx, pgwg, pgwu, pgg, pgu, pgh, pg, pu, pwg, pwu, px, yvec, ndat, xvec, act,
+                                 leaky_alpha, acc_x, acc_w, s);
     if (ndat * yvec > 0)
         KAI_TRY(gated_apply_backward(st, pgg, pgu, pgh, pg, pu, ndat * yvec, act, leaky_alpha, s));
-    if (pgx) {
-        KAI_TRY(kai_sgemm(device, KAI_GEMM_NN, pgx, pgg, pwg, ndat, xvec, yvec, xvec, acc_x, nullptr, KAI_ACT_NONE, nullptr,
-                          KAI_PATH_AUTO, stream));
-        KAI_TRY(kai_sgemm(device, KAI_GEMM_NN, pgx, pgu, pwu, ndat, xvec, yvec, xvec, 1, nullptr, KAI_ACT_NONE, nullptr,
-                          KAI_PATH_AUTO, stream));
-    }
-    if (pgwg) {
-        KAI_TRY(kai_sgemm(device, KAI_GEMM_TN, pgwg, pgg, px, yvec, xvec, ndat, xvec, acc_w, nullptr, KAI_ACT_NONE, nullptr,
-                          KAI_PATH_AUTO, stream));
-        KAI_TRY(kai_sgemm(device, KAI_GEMM_TN, pgwu, pgu, px, yvec, xvec, ndat, xvec, acc_w, nullptr, KAI_ACT_NONE, nullptr,
-                          KAI_PATH_AUTO, stream));
-    }
-    return KAI_OK;
+    const bool want_x = pgx != nullptr && ndat > 0, want_w = pgwg != nullptr && yvec > 0;
+    if (xvec == 0 || (!want_x && !want_w)) return KAI_OK;
+    return gated_backward_mma(st, want_x ? pgx : nullptr, want_w ? pgwg : nullptr, want_w ? pgwu : nullptr, pgg, pgu, pwg, pwu, px,
+                              yvec, ndat, xvec, acc_x, acc_w, s);
 }
 
 // ---- losses on rows of logits ----------------------------------------------------------------

@@ -106,6 +106,18 @@ struct TcParams {
     int xb = 0;        // channels per box
     int xblocks = 1;   // channel blocks per column shift
     int mixed = 0;     // second planes hold bf16 cross-term operands: one TF32 and one BF16 MMA per K step
+    // Rows from c_split on belong to a second output, c2 (the two weight gradients of a gated layer).
+    float* c2 = nullptr;
+    int64_t c_split = 0;
+    // Gated layer: the tile's columns are BN / 2 of the gate and the same BN / 2 of the up projection; N counts hidden units,
+    // c receives act(g + bias) * (u + bias_u), save_g / save_u the two factors' sums (may be null).
+    float* save_g = nullptr;
+    float* save_u = nullptr;
+    const float* bias_u = nullptr;
+
+    __device__ __forceinline__ float* out(int64_t row, int64_t n) const {
+        return (c2 != nullptr && row >= c_split) ? c2 + (row - c_split) * ldc + n : c + row * ldc + n;
+    }
 };
 
 // The tensor maps of the tap-row form: per kernel row one hi and one lo map whose base is that row's offset.
@@ -193,7 +205,7 @@ __device__ __forceinline__ void store_chunk(const TcParams& p, const WorkItem& i
     const int64_t row = static_cast<int64_t>(it.m_blk) * BM + row_in_tile;
     const int64_t n0 = static_cast<int64_t>(it.n_blk) * BN + col_in_tile;
     if (row >= p.M || n0 >= p.N) return;
-    float* out = p.c + row * p.ldc + n0;
+    float* out = p.out(row, n0);
     const bool plain = !p.bias && !p.accumulate && p.act == KAI_ACT_NONE;
     const int64_t ncols = (p.N - n0 < 32) ? (p.N - n0) : 32;
 #pragma unroll
@@ -223,13 +235,114 @@ __device__ __forceinline__ void store_chunk(const TcParams& p, const WorkItem& i
     }
 }
 
+// Accumulator column at which chunk `cc` (32 columns) of an epilogue warp's half begins.  Plain tiles: the half's columns in
+// order.  Gated tiles: the first half of the chunks is gate columns, the second the up columns of the same hidden units,
+// so that a thread holds both factors of its outputs.
+template <int BN, bool GATED>
+__device__ __forceinline__ int chunk_col(int half, int cc) {
+    constexpr int HALF = BN / 2, Q = BN / 4;
+    if (!GATED) return half * HALF + cc * 32;
+    return (cc * 32 < Q) ? half * Q + cc * 32 : HALF + half * Q + (cc * 32 - Q);
+}
+
+// Outputs of 32 consecutive hidden units of one row of a gated tile.
+__device__ __forceinline__ void store_gated4(const TcParams& p, int64_t row, int64_t n0, const float* g, const float* u, bool vec_ok,
+                                             float alpha) {
+    const int64_t left = p.N - n0;
+    float gv[4], uv[4], hv[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        gv[i] = g[i];
+        uv[i] = u[i];
+        if (i < left) {
+            if (p.bias) gv[i] += __ldg(p.bias + n0 + i);
+            if (p.bias_u) uv[i] += __ldg(p.bias_u + n0 + i);
+        }
+        hv[i] = act_forward(p.act, gv[i], alpha) * uv[i];
+    }
+    const int64_t at = row * p.ldc + n0;
+    if (vec_ok && left >= 4) {
+        *reinterpret_cast<float4*>(p.c + at) = make_float4(hv[0], hv[1], hv[2], hv[3]);
+        if (p.save_g) {
+            *reinterpret_cast<float4*>(p.save_g + at) = make_float4(gv[0], gv[1], gv[2], gv[3]);
+            *reinterpret_cast<float4*>(p.save_u + at) = make_float4(uv[0], uv[1], uv[2], uv[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i < left) {
+                p.c[at + i] = hv[i];
+                if (p.save_g) { p.save_g[at + i] = gv[i]; p.save_u[at + i] = uv[i]; }
+            }
+        }
+    }
+}
+__device__ __forceinline__ bool gated_vec_ok(const TcParams& p) {
+    return (p.ldc & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.c) | reinterpret_cast<uintptr_t>(p.save_g) |
+                                 reinterpret_cast<uintptr_t>(p.save_u)) & 15) == 0;
+}
+// An epilogue warp's half of a finished gated tile: acc holds BN / 4 gate sums and the up sums of the same hidden units.  They pass
+// through the warp's 4 KB of shared memory, 16 units at a time, so that the activation stands four times in the
+// program and not once per register (64 copies of its nine cases cost 60 us of instruction fetches per call), and so that
+// neighbouring lanes store neighbouring values.
+constexpr int kGatedStageBytes = kEpiWarps * 4096;
+template <int BN>
+__device__ __forceinline__ void store_gated(const TcParams& p, const WorkItem& it, int row0, int half, const float* acc, float* stage,
+                                            float alpha) {
+    constexpr int Q = BN / 4;
+    const int lane = threadIdx.x & 31;
+    const int64_t n_half = static_cast<int64_t>(it.n_blk) * (BN / 2) + half * Q;
+#pragma unroll
+    for (int c = 0; c < Q / 16; ++c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {          // 16-byte piece i of this lane's row: four gate pieces, four up pieces
+            const float* v = (i < 4) ? acc + c * 16 + 4 * i : acc + Q + c * 16 + 4 * (i - 4);
+            *reinterpret_cast<float4*>(stage + lane * 32 + ((i ^ (lane & 7)) << 2)) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        __syncwarp();
+        const int col = lane & 15;
+        const int64_t n = n_half + c * 16 + col;
+        if (n < p.N) {
+            const float bg = p.bias ? __ldg(p.bias + n) : 0.0f, bu = p.bias_u ? __ldg(p.bias_u + n) : 0.0f;
+#pragma unroll 2
+            for (int r = lane >> 4; r < 32; r += 2) {
+                const int64_t row = static_cast<int64_t>(it.m_blk) * BM + row0 + r;
+                if (row >= p.M) break;
+                const float* at = stage + r * 32 + (col & 3);
+                const float g = at[((col >> 2) ^ (r & 7)) << 2] + bg, u = at[((4 + (col >> 2)) ^ (r & 7)) << 2] + bu;
+                const int64_t o = row * p.ldc + n;
+                p.c[o] = act_forward(p.act, g, alpha) * u;
+                if (p.save_g) { p.save_g[o] = g; p.save_u[o] = u; }
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// An epilogue warp's half of a finished tile (or of a piece of one).
+template <int BN, bool GATED>
+__device__ __forceinline__ void store_half(const TcParams& p, const WorkItem& it, int row0, int half, const float* acc, bool vec_ok,
+                                           float alpha, uint8_t* stages) {
+    constexpr int HALF = BN / 2;
+    if (GATED && it.slot < 0) {
+        store_gated<BN>(p, it, row0, half, acc, reinterpret_cast<float*>(stages) + ((threadIdx.x >> 5) - 2) * 1024, alpha);
+    } else {
+#pragma unroll
+        for (int cc = 0; cc < HALF / 32; ++cc)
+            store_chunk<BN>(p, it, row0 + (threadIdx.x & 31), chunk_col<BN, GATED>(half, cc), &acc[cc * 32], vec_ok, alpha);
+    }
+}
+
 // ---------------------------------------------------------------------------------------
 // The GEMM kernel
 // ---------------------------------------------------------------------------------------
-template <int BN, int BK, int KH>
+// GATED: the B tile's first BN / 2 rows come from map_b_* (gate weights), the others from map_u_* (up weights), at the
+// same hidden units.
+template <int BN, int BK, int KH, bool GATED = false>
 __device__ __forceinline__ void
 gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const CUtensorMap& map_b_hi,
-                 const CUtensorMap& map_b_lo, const TapMaps* taps, const TcParams& p) {
+                 const CUtensorMap& map_b_lo, const TapMaps* taps, const TcParams& p, const CUtensorMap* map_u_hi = nullptr,
+                 const CUtensorMap* map_u_lo = nullptr) {
     using C = Cfg<BN, BK>;
     extern __shared__ uint8_t smem_raw[];
     // Swizzled tiles need their base on a 1024-byte boundary.
@@ -302,7 +415,14 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
                     const int k0 = kb * BK;
                     tma_load_2d(smem_u32(base), &map_a_hi, full, k0, row_a);
                     tma_load_2d(smem_u32(base + C::A_BYTES), &map_a_lo, full, k0, row_a);
-                    if (KH == 0) {
+                    if (GATED) {
+                        constexpr int SUB = C::B_BYTES / 2;
+                        const int unit = it.n_blk * (BN / 2);
+                        tma_load_2d(smem_u32(base + 2 * C::A_BYTES), &map_b_hi, full, k0, unit);
+                        tma_load_2d(smem_u32(base + 2 * C::A_BYTES + SUB), map_u_hi, full, k0, unit);
+                        tma_load_2d(smem_u32(base + 2 * C::A_BYTES + C::B_BYTES), &map_b_lo, full, k0, unit);
+                        tma_load_2d(smem_u32(base + 2 * C::A_BYTES + C::B_BYTES + SUB), map_u_lo, full, k0, unit);
+                    } else if (KH == 0) {
                         tma_load_2d(smem_u32(base + 2 * C::A_BYTES), &map_b_hi, full, k0, row_b);
                         tma_load_2d(smem_u32(base + 2 * C::A_BYTES + C::B_BYTES), &map_b_lo, full, k0, row_b);
                     } else {
@@ -381,7 +501,7 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
         const int quarter = warp & 3;
         const int half = (warp - 2) >> 2;
         const float alpha = (p.leaky_alpha != nullptr) ? __ldg(p.leaky_alpha) : 0.0f;
-        const bool vec_ok = (p.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
+        const bool vec_ok = (p.ldc & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.c) | reinterpret_cast<uintptr_t>(p.c2)) & 15) == 0;
         int acc_buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -394,12 +514,11 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
                 ok = mbar_wait(smem_u32(&tmem_full_bar[acc_buf]), acc_phase, abort_flag, p.status, 4);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                       static_cast<uint32_t>(acc_buf * BN + half * HALF);
+                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc_buf * BN);
 #pragma unroll
                 for (int cc = 0; cc < HALF / 32; ++cc) {
                     uint32_t r[32];
-                    tmem_ld32(taddr + static_cast<uint32_t>(cc * 32), r);
+                    tmem_ld32(taddr + static_cast<uint32_t>(chunk_col<BN, GATED>(half, cc)), r);
                     tmem_ld_wait(r);
                     if (first_chunk) {
 #pragma unroll
@@ -417,9 +536,7 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
                 if (acc_buf == 0) acc_phase ^= 1u;
             }
             if (!ok) break;
-#pragma unroll
-            for (int cc = 0; cc < HALF / 32; ++cc)
-                store_chunk<BN>(p, it, quarter * 32 + lane, half * HALF + cc * 32, &acc[cc * 32], vec_ok, alpha);
+            store_half<BN, GATED>(p, it, quarter * 32, half, acc, vec_ok, alpha, smem + C::STAGES * C::STAGE_BYTES + 256);
         }
     }
 
@@ -447,6 +564,16 @@ gemm_3xtf32_kernel(const __grid_constant__ CUtensorMap map_a_hi,
                    const __grid_constant__ CUtensorMap map_b_hi,
                    const __grid_constant__ CUtensorMap map_b_lo, const TcParams p) {
     gemm_3xtf32_body<BN, BK, 0>(map_a_hi, map_a_lo, map_b_hi, map_b_lo, nullptr, p);
+}
+
+// The gated layer's projections: both weights in one tile, h = act(g) * u in the epilogue.
+template <int BN, int BK>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_3xtf32_gated_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __grid_constant__ CUtensorMap map_a_lo,
+                         const __grid_constant__ CUtensorMap map_g_hi, const __grid_constant__ CUtensorMap map_g_lo,
+                         const __grid_constant__ CUtensorMap map_u_hi, const __grid_constant__ CUtensorMap map_u_lo,
+                         const TcParams p) {
+    gemm_3xtf32_body<BN, BK, 0, true>(map_a_hi, map_a_lo, map_g_hi, map_g_lo, nullptr, p, &map_u_hi, &map_u_lo);
 }
 
 // The same kernel with the B operand in tap-row form (see TcParams): the kernel gradient of a convolution read
@@ -491,11 +618,13 @@ struct PairCfg {
     static constexpr int TMEM_COLS = 512;               // two accumulator buffers of 256 columns
 };
 
-template <int BK>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-gemm_3xtf32_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __grid_constant__ CUtensorMap map_a_lo,
-                        const __grid_constant__ CUtensorMap map_b_hi, const __grid_constant__ CUtensorMap map_b_lo,
-                        const TcParams p) {
+// GATED: the leader's half of the B tile is 128 rows of the gate weights (map_b_*), the other CTA's the same 128 rows of the up
+// weights, so that the gate's sums lie in columns 0 to 127 of the accumulator and the up projection's behind them.
+template <int BK, bool GATED>
+__device__ __forceinline__ void
+gemm_pair_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const CUtensorMap& map_b_hi,
+               const CUtensorMap& map_b_lo, const TcParams& p, const CUtensorMap* map_u_hi = nullptr,
+               const CUtensorMap* map_u_lo = nullptr) {
     using C = PairCfg<BK>;
     constexpr int BN = C::BNP;
     extern __shared__ uint8_t smem_raw[];
@@ -557,7 +686,9 @@ gemm_3xtf32_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __gr
                 int pm, n_blk;
                 tile_coords(p, t, pm, n_blk);
                 const int row_a = (2 * pm + static_cast<int>(rank)) * BM;
-                const int row_b = n_blk * BN + static_cast<int>(rank) * (BN / 2);
+                const int row_b = GATED ? n_blk * (BN / 2) : n_blk * BN + static_cast<int>(rank) * (BN / 2);
+                const CUtensorMap* b_hi_map = (GATED && rank != 0) ? map_u_hi : &map_b_hi;
+                const CUtensorMap* b_lo_map = (GATED && rank != 0) ? map_u_lo : &map_b_lo;
                 for (int kb = 0; kb < p.kb_total; ++kb) {
                     ok = mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag, p.status, 5);
                     if (!ok) break;
@@ -567,8 +698,8 @@ gemm_3xtf32_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __gr
                     const int k0 = kb * BK;
                     tma_load_2d_pair(base, &map_a_hi, full, k0, row_a);
                     tma_load_2d_pair(base + C::T_BYTES, &map_a_lo, full, k0, row_a);
-                    tma_load_2d_pair(base + 2 * C::T_BYTES, &map_b_hi, full, k0, row_b);
-                    tma_load_2d_pair(base + 3 * C::T_BYTES, &map_b_lo, full, k0, row_b);
+                    tma_load_2d_pair(base + 2 * C::T_BYTES, b_hi_map, full, k0, row_b);
+                    tma_load_2d_pair(base + 3 * C::T_BYTES, b_lo_map, full, k0, row_b);
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -631,7 +762,7 @@ gemm_3xtf32_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __gr
         const int quarter = warp & 3;
         const int half = (warp - 2) >> 2;
         const float alpha = (p.leaky_alpha != nullptr) ? __ldg(p.leaky_alpha) : 0.0f;
-        const bool vec_ok = (p.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
+        const bool vec_ok = (p.ldc & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.c) | reinterpret_cast<uintptr_t>(p.c2)) & 15) == 0;
         int acc_buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -647,12 +778,11 @@ gemm_3xtf32_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __gr
                 ok = mbar_wait(smem_u32(&tmem_full_bar[acc_buf]), acc_phase, abort_flag, p.status, 8);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                       static_cast<uint32_t>(acc_buf * BN + half * HALF);
+                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc_buf * BN);
 #pragma unroll
                 for (int cc = 0; cc < HALF / 32; ++cc) {
                     uint32_t r[32];
-                    tmem_ld32(taddr + static_cast<uint32_t>(cc * 32), r);
+                    tmem_ld32(taddr + static_cast<uint32_t>(chunk_col<BN, GATED>(half, cc)), r);
                     tmem_ld_wait(r);
                     if (first_chunk) {
 #pragma unroll
@@ -670,9 +800,7 @@ gemm_3xtf32_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __gr
                 if (acc_buf == 0) acc_phase ^= 1u;
             }
             if (!ok) break;
-#pragma unroll
-            for (int cc = 0; cc < HALF / 32; ++cc)
-                store_chunk<BN>(p, it, quarter * 32 + lane, half * HALF + cc * 32, &acc[cc * 32], vec_ok, alpha);
+            store_half<BN, GATED>(p, it, quarter * 32, half, acc, vec_ok, alpha, smem + C::STAGES * C::STAGE_BYTES + 256);
         }
     }
 
@@ -690,6 +818,21 @@ gemm_3xtf32_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __gr
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
     }
+}
+
+template <int BK>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gemm_3xtf32_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __grid_constant__ CUtensorMap map_a_lo,
+                        const __grid_constant__ CUtensorMap map_b_hi, const __grid_constant__ CUtensorMap map_b_lo,
+                        const TcParams p) {
+    gemm_pair_body<BK, false>(map_a_hi, map_a_lo, map_b_hi, map_b_lo, p);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gemm_3xtf32_gated_pair_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __grid_constant__ CUtensorMap map_a_lo,
+                              const __grid_constant__ CUtensorMap map_g_hi, const __grid_constant__ CUtensorMap map_g_lo,
+                              const __grid_constant__ CUtensorMap map_u_hi, const __grid_constant__ CUtensorMap map_u_lo,
+                              const TcParams p) {
+    gemm_pair_body<32, true>(map_a_hi, map_a_lo, map_g_hi, map_g_lo, p, &map_u_hi, &map_u_lo);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -737,6 +880,42 @@ __device__ __forceinline__ void store_cross4(float* row, int64_t k, const float 
 // With hi == nullptr only the lo plane is written, against the TRUNCATED high part
 // (a & 0xffffe000): the GEMM then reads the caller's fp32 matrix itself as the hi plane, the
 // tensor core ignoring the low 13 mantissa bits of a TF32 operand.
+__device__ __forceinline__ void split_quad(const float* __restrict__ src, int64_t r, int64_t k, int64_t cols, int64_t ld,
+                                           float* __restrict__ hi, float* __restrict__ lo, int64_t kp, int vec_src, int xside) {
+    float v[4];
+    const float* s = src + r * ld + k;
+    if (vec_src && k + 3 < cols) {
+        const float4 t = *reinterpret_cast<const float4*>(s);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (k + j < cols) ? s[j] : 0.0f;
+    }
+    float h[4], l[4];
+    if (hi != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_tf32(v[j], h[j], l[j]);
+        *reinterpret_cast<float4*>(hi + r * kp + k) = make_float4(h[0], h[1], h[2], h[3]);
+        if (xside) { store_cross4(lo + r * kp, k, v, h, xside); return; }
+    } else {
+        if (xside) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[j] = __uint_as_float(__float_as_uint(v[j]) & 0xFFFFE000u);
+            store_cross4(lo + r * kp, k, v, h, xside);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float t = __uint_as_float(__float_as_uint(v[j]) & 0xFFFFE000u);
+            const float rest = isfinite(v[j]) ? (v[j] - t) : 0.0f;
+            uint32_t lw;
+            asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lw) : "f"(rest));
+            l[j] = __uint_as_float(lw);
+        }
+    }
+    *reinterpret_cast<float4*>(lo + r * kp + k) = make_float4(l[0], l[1], l[2], l[3]);
+}
+
 __global__ void split_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t cols,
                                   int64_t ld, float* __restrict__ hi, float* __restrict__ lo,
                                   int64_t kp, int vec_src, int xside) {
@@ -745,39 +924,7 @@ __global__ void split_rows_kernel(const float* __restrict__ src, int64_t rows, i
     for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t r = i / quads_per_row;
-        const int64_t k = (i - r * quads_per_row) << 2;
-        float v[4];
-        const float* s = src + r * ld + k;
-        if (vec_src && k + 3 < cols) {
-            const float4 t = *reinterpret_cast<const float4*>(s);
-            v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = (k + j < cols) ? s[j] : 0.0f;
-        }
-        float h[4], l[4];
-        if (hi != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split_tf32(v[j], h[j], l[j]);
-            *reinterpret_cast<float4*>(hi + r * kp + k) = make_float4(h[0], h[1], h[2], h[3]);
-            if (xside) { store_cross4(lo + r * kp, k, v, h, xside); continue; }
-        } else {
-            if (xside) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) h[j] = __uint_as_float(__float_as_uint(v[j]) & 0xFFFFE000u);
-                store_cross4(lo + r * kp, k, v, h, xside);
-                continue;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float t = __uint_as_float(__float_as_uint(v[j]) & 0xFFFFE000u);
-                const float rest = isfinite(v[j]) ? (v[j] - t) : 0.0f;
-                uint32_t lw;
-                asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lw) : "f"(rest));
-                l[j] = __uint_as_float(lw);
-            }
-        }
-        *reinterpret_cast<float4*>(lo + r * kp + k) = make_float4(l[0], l[1], l[2], l[3]);
+        split_quad(src, r, (i - r * quads_per_row) << 2, cols, ld, hi, lo, kp, vec_src, xside);
     }
 }
 
@@ -821,6 +968,34 @@ split_lo_flat_kernel(const float4* __restrict__ a, const float4* __restrict__ b,
     }
 }
 
+// A 64 x 64 tile of some matrix in shared memory, tile[row][column]: writes its transpose into K-major planes [dst_rows][pitch],
+// dst row = c0 + column, k = k_off + r0 + row for r0 + row < k_end (a multiple of 4; rows beyond the source hold zeros).
+__device__ __forceinline__ void store_transposed(const float (&tile)[64][65], int64_t r0, int64_t c0, int64_t dst_rows, int64_t k_end,
+                                                 float* __restrict__ hi, float* __restrict__ lo, int64_t pitch, int64_t k_off,
+                                                 int64_t dst_row0, int xside) {
+    const int q = threadIdx.x & 15, l = threadIdx.x >> 4;
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+        const int i = l + 16 * pass;        // dst row inside the tile (= source column)
+        const int64_t dr = c0 + i;
+        const int64_t dk = r0 + 4 * q;      // dst k (= source row), 4 at a time
+        if (dr < dst_rows && dk < k_end) {
+            float* h_at = hi + (dst_row0 + dr) * pitch;
+            float* l_at = lo + (dst_row0 + dr) * pitch;
+            float h[4], lw[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split_tf32(tile[4 * q + e][i], h[e], lw[e]);  // zero beyond the source
+            *reinterpret_cast<float4*>(h_at + k_off + dk) = make_float4(h[0], h[1], h[2], h[3]);
+            if (xside) {
+                const float v[4] = {tile[4 * q][i], tile[4 * q + 1][i], tile[4 * q + 2][i], tile[4 * q + 3][i]};
+                store_cross4(l_at, k_off + dk, v, h, xside);
+            } else {
+                *reinterpret_cast<float4*>(l_at + k_off + dk) = make_float4(lw[0], lw[1], lw[2], lw[3]);
+            }
+        }
+    }
+}
+
 // Transposing variant: src is [src_rows][src_cols] (row stride ld); dst planes are
 // [src_cols][kp] with the reduction index = src row.  64 x 64 tiles through shared memory,
 // 16-byte loads when the source allows them and 16-byte stores always (kp % 4 == 0).
@@ -855,24 +1030,7 @@ split_transpose_kernel(const float* __restrict__ src, int64_t src_rows, int64_t 
         for (int e = 0; e < 4; ++e) tile[i][4 * q + e] = v[e];
     }
     __syncthreads();
-#pragma unroll
-    for (int pass = 0; pass < 4; ++pass) {
-        const int i = l + 16 * pass;        // dst row inside the tile (= source column)
-        const int64_t dr = c0 + i;
-        const int64_t dk = r0 + 4 * q;      // dst k (= source row), 4 at a time
-        if (dr < src_cols && dk < kp) {
-            float h[4], lw[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split_tf32(tile[4 * q + e][i], h[e], lw[e]);  // zero beyond src_rows
-            *reinterpret_cast<float4*>(hi + dr * kp + dk) = make_float4(h[0], h[1], h[2], h[3]);
-            if (xside) {
-                const float v[4] = {tile[4 * q][i], tile[4 * q + 1][i], tile[4 * q + 2][i], tile[4 * q + 3][i]};
-                store_cross4(lo + dr * kp, dk, v, h, xside);
-            } else {
-                *reinterpret_cast<float4*>(lo + dr * kp + dk) = make_float4(lw[0], lw[1], lw[2], lw[3]);
-            }
-        }
-    }
+    store_transposed(tile, r0, c0, src_cols, kp, hi, lo, kp, 0, 0, xside);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -890,7 +1048,7 @@ fixup_kernel(const TcParams p) {
     const int r_first = (j * p.kb_total) / p.sk_per;
     const int r_last = ((j + 1) * p.kb_total - 1) / p.sk_per;
     const float alpha = (p.leaky_alpha != nullptr) ? __ldg(p.leaky_alpha) : 0.0f;
-    const bool vec_ok = (p.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
+    const bool vec_ok = (p.ldc & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.c) | reinterpret_cast<uintptr_t>(p.c2)) & 15) == 0;
     const bool plain = !p.bias && !p.accumulate && p.act == KAI_ACT_NONE;
     constexpr int QUADS = BM * BN / 4, PER_BLOCK = QUADS / FIXUP_PARTS;
     static_assert(QUADS % FIXUP_PARTS == 0, "tile elements divide among the blocks");
@@ -915,7 +1073,7 @@ fixup_kernel(const TcParams p) {
             }
         }
         float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        float* out = p.c + row * p.ldc + n0;
+        float* out = p.out(row, n0);
         const int64_t ncols = (p.N - n0 < 4) ? (p.N - n0) : 4;
         if (!plain) {
 #pragma unroll
@@ -936,6 +1094,184 @@ fixup_kernel(const TcParams p) {
                 if (i < ncols) out[i] = v[i];
         }
     }
+}
+
+// The same for a gated tile (128 gate columns, then the up columns of the same units).
+__global__ void __launch_bounds__(256)
+fixup_gated_kernel(const TcParams p) {
+    constexpr int BN = 256;
+    const int j = blockIdx.x;
+    int m_blk, n_blk;
+    tile_coords(p, p.full_tiles + j, m_blk, n_blk);
+    const int r_first = (j * p.kb_total) / p.sk_per;
+    const int r_last = ((j + 1) * p.kb_total - 1) / p.sk_per;
+    const float alpha = (p.leaky_alpha != nullptr) ? __ldg(p.leaky_alpha) : 0.0f;
+    const bool vec_ok = gated_vec_ok(p);
+    constexpr int QUADS = BM * BN / 8, PER_BLOCK = QUADS / FIXUP_PARTS;
+    for (int q = blockIdx.y * PER_BLOCK + threadIdx.x; q < static_cast<int>(blockIdx.y + 1) * PER_BLOCK; q += 256) {
+        const int row_in = q / (BN / 8), col_in = (q % (BN / 8)) * 4;
+        const int64_t row = static_cast<int64_t>(m_blk) * BM + row_in;
+        const int64_t n0 = static_cast<int64_t>(n_blk) * (BN / 2) + col_in;
+        if (row >= p.M || n0 >= p.N) continue;
+        float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+        for (int r = r_first; r <= r_last; r += 4) {      // loads first, adds in range order
+            float4 t[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float* at = p.partial + (static_cast<int64_t>(min(r + e, r_last) + j) * BM + row_in) * BN + col_in;
+                t[2 * e] = __ldcs(reinterpret_cast<const float4*>(at));
+                t[2 * e + 1] = __ldcs(reinterpret_cast<const float4*>(at + BN / 2));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (r + e <= r_last) {
+                    g.x += t[2 * e].x; g.y += t[2 * e].y; g.z += t[2 * e].z; g.w += t[2 * e].w;
+                    u.x += t[2 * e + 1].x; u.y += t[2 * e + 1].y; u.z += t[2 * e + 1].z; u.w += t[2 * e + 1].w;
+                }
+            }
+        }
+        const float gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
+        store_gated4(p, row, n0, gv, uv, vec_ok, alpha);
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Gated layer: operand planes, one launch each way
+// ---------------------------------------------------------------------------------------
+// Row-major matrices of one width (x and both weights) into planes; blockIdx.y picks the matrix.
+struct RowJobs {
+    const float* src[3];
+    float* hi[3];            // nullptr: the matrix itself serves as hi plane
+    float* lo[3];
+    int64_t rows[3];
+    int64_t cols, kp;
+    int vec[3], xside[3];
+};
+__global__ void __launch_bounds__(256)
+split_row_jobs_kernel(const RowJobs p) {
+    const int j = blockIdx.y;
+    const int64_t quads = p.kp >> 2, total = p.rows[j] * quads;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / quads;
+        split_quad(p.src[j], r, (i - r * quads) << 2, p.cols, p.cols, p.hi[j], p.lo[j], p.kp, p.vec[j], p.xside[j]);
+    }
+}
+
+// Everything the two products of the backward call read, from one pass over the operands.  With gg = gh u act'(g) and
+// gu = gh act(g) (computed once per value, written out as well):
+//   d planes   [ndat][2 fp]   gg | gu of a row, each padded with zeros to fp values           left operand of pgx
+//   w planes   [xvec][2 fp]   the columns of pwg | pwu                                        right operand of pgx
+//   dt planes  [2 yvec][mp]   the columns of gg, then those of gu                             left operand of both pgw
+//   xt planes  [xvec][mp]     the columns of px                                               right operand of both pgw
+// 64 x 64 tiles, transposed through shared memory; blocks [0, d_tiles) are tiles of gh / g / u, the others of a weight or of px.
+struct BackParams {
+    const float *gh, *g, *u, *wg, *wu, *x, *leaky_alpha;
+    float *gg, *gu;
+    float *d_hi, *d_lo, *dt_hi, *dt_lo, *w_hi, *w_lo, *xt_hi, *xt_lo;   // null where not wanted
+    int64_t ndat, xvec, yvec, fp, mp;
+    int d_tiles, w_tiles, f_tiles, k_tiles;     // f_tiles, k_tiles: tiles along yvec (padded to fp) and xvec
+    int act, mixed_x, mixed_w, vec;             // vec: every row of every operand begins on a 16-byte boundary
+};
+__device__ __forceinline__ void load_tile(float (&tile)[64][65], const float* __restrict__ src, int64_t rows, int64_t cols, int64_t r0,
+                                          int64_t c0, int vec) {
+    const int q = threadIdx.x & 15, l = threadIdx.x >> 4;
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+        const int64_t r = r0 + l + 16 * pass, c = c0 + 4 * q;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (r < rows) {
+            if (vec && c + 3 < cols) {
+                const float4 t = *reinterpret_cast<const float4*>(src + r * cols + c);
+                v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < cols) v[e] = src[r * cols + c + e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[l + 16 * pass][4 * q + e] = v[e];
+    }
+}
+__global__ void __launch_bounds__(256)
+gated_backward_planes_kernel(const BackParams p) {
+    __shared__ float tile[2][64][65];
+    int b = blockIdx.x;
+    if (b >= p.d_tiles) {
+        b -= p.d_tiles;
+        const bool weight = b < 2 * p.w_tiles;
+        const int which = weight ? b / p.w_tiles : 0;
+        const int t = weight ? b % p.w_tiles : b - 2 * p.w_tiles;
+        const int64_t r0 = static_cast<int64_t>(t / p.k_tiles) * 64, c0 = static_cast<int64_t>(t % p.k_tiles) * 64;
+        if (weight) {
+            load_tile(tile[0], which ? p.wu : p.wg, p.yvec, p.xvec, r0, c0, p.vec);
+            __syncthreads();
+            store_transposed(tile[0], r0, c0, p.xvec, p.fp, p.w_hi, p.w_lo, 2 * p.fp, which * p.fp, 0, p.mixed_x ? 2 : 0);
+        } else {
+            load_tile(tile[0], p.x, p.ndat, p.xvec, r0, c0, p.vec);
+            __syncthreads();
+            store_transposed(tile[0], r0, c0, p.xvec, p.mp, p.xt_hi, p.xt_lo, p.mp, 0, 0, p.mixed_w ? 2 : 0);
+        }
+        return;
+    }
+    const float alpha = (p.leaky_alpha != nullptr) ? __ldg(p.leaky_alpha) : 0.0f;
+    const int64_t r0 = static_cast<int64_t>(b / p.f_tiles) * 64, c0 = static_cast<int64_t>(b % p.f_tiles) * 64;
+    const int q = threadIdx.x & 15, l = threadIdx.x >> 4;
+#pragma unroll 1
+    for (int pass = 0; pass < 4; ++pass) {
+        const int i = l + 16 * pass;
+        const int64_t r = r0 + i, c = c0 + 4 * q, at = r * p.yvec + c;
+        float d[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+        const bool whole = p.vec && c + 3 < p.yvec;
+        if (r < p.ndat) {
+            if (whole) {
+                *reinterpret_cast<float4*>(d) = *reinterpret_cast<const float4*>(p.gh + at);
+                *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(p.g + at);
+                *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(p.u + at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < p.yvec) { d[e] = p.gh[at + e]; g[e] = p.g[at + e]; u[e] = p.u[at + e]; }
+            }
+        }
+        float gg[4], gu[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = r < p.ndat && c + e < p.yvec;
+            const float2 v = act_value_slope(p.act, g[e], alpha);
+            gg[e] = in ? d[e] * u[e] * v.y : 0.0f;
+            gu[e] = in ? d[e] * v.x : 0.0f;
+            tile[0][i][4 * q + e] = gg[e];
+            tile[1][i][4 * q + e] = gu[e];
+        }
+        if (r < p.ndat) {
+            if (whole) {
+                *reinterpret_cast<float4*>(p.gg + at) = *reinterpret_cast<float4*>(gg);
+                *reinterpret_cast<float4*>(p.gu + at) = *reinterpret_cast<float4*>(gu);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < p.yvec) { p.gg[at + e] = gg[e]; p.gu[at + e] = gu[e]; }
+            }
+            if (p.d_hi != nullptr && c < p.fp) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float* v = half ? gu : gg;
+                    const int64_t k = half * p.fp + c;
+                    float h[4], lw[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split_tf32(v[e], h[e], lw[e]);
+                    *reinterpret_cast<float4*>(p.d_hi + r * 2 * p.fp + k) = make_float4(h[0], h[1], h[2], h[3]);
+                    if (p.mixed_x) store_cross4(p.d_lo + r * 2 * p.fp, k, v, h, 1);
+                    else *reinterpret_cast<float4*>(p.d_lo + r * 2 * p.fp + k) = make_float4(lw[0], lw[1], lw[2], lw[3]);
+                }
+            }
+        }
+    }
+    if (p.dt_hi == nullptr) return;
+    __syncthreads();
+    store_transposed(tile[0], r0, c0, p.yvec, p.mp, p.dt_hi, p.dt_lo, p.mp, 0, 0, p.mixed_w ? 1 : 0);
+    store_transposed(tile[1], r0, c0, p.yvec, p.mp, p.dt_hi, p.dt_lo, p.mp, 0, p.yvec, p.mixed_w ? 1 : 0);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1113,7 +1449,7 @@ static int64_t max_slots(int64_t tiles, int sms, int forced) {
     return rem > 0 ? rem + sms : 0;
 }
 
-static int plan_tc(const DeviceState* st, int64_t M, int64_t N, int64_t K, TcPlan* out, int force_bn = 0) {
+static int plan_tc(const DeviceState* st, int64_t M, int64_t N, int64_t K, TcPlan* out, int force_bn = 0, bool gated = false) {
     if (M >= (int64_t(1) << 31) || N >= (int64_t(1) << 31) || K >= (int64_t(1) << 31))
         return fail(KAI_E_TOO_LARGE, "gemm_tc: a dimension exceeds 2^31-1");
     Options& opt = options();
@@ -1122,6 +1458,7 @@ static int plan_tc(const DeviceState* st, int64_t M, int64_t N, int64_t K, TcPla
     pl.bk = (opt.tc_bk.load() == 32) ? 32 : 16;
     pl.bn = (opt.tc_bn.load() == 128) ? 128 : 256;
     if (N <= 128) pl.bn = 128;
+    if (gated) { pl.bn = 256; pl.bk = 16; }     // N counts the columns of both projections, in whole tiles
     if (force_bn > 0) { pl.bn = force_bn; pl.bk = 16; }
     pl.tiles_m = static_cast<int>((M + BM - 1) / BM);
     pl.tiles_n = static_cast<int>((N + pl.bn - 1) / pl.bn);
@@ -1158,7 +1495,7 @@ static int plan_tc(const DeviceState* st, int64_t M, int64_t N, int64_t K, TcPla
         const int pairs = sms / 2;
         if (tiles_p * 2 >= pairs) {      // from half a round on: the same share of SMs is busy as with 128-row tiles
             pl.pair = true;
-            pl.bk = (opt.tc_pair_bk.load() == 16) ? 16 : 32;
+            pl.bk = (!gated && opt.tc_pair_bk.load() == 16) ? 16 : 32;
             pl.kb_total = static_cast<int>((K + pl.bk - 1) / pl.bk);
             pl.tiles_m = tiles_mp;
             pl.full_tiles = static_cast<int>(tiles_p);
@@ -1212,16 +1549,54 @@ static int plan_tc(const DeviceState* st, int64_t M, int64_t N, int64_t K, TcPla
     return KAI_OK;
 }
 
+// The second projection of a gated layer, and where its epilogue's other outputs go.
+struct GatedOut {
+    const float* u_hi;
+    const float* u_lo;
+    float* g;
+    float* u;
+    const float* bias_u;
+};
+
+static int launch_gemm_gated(const CUtensorMap maps[6], const TcParams& p, bool pair, int grid, cudaStream_t s) {
+    using C = Cfg<256, 16>;
+    constexpr int smem = C::STAGES * C::STAGE_BYTES + 1024 + 256 + kGatedStageBytes;
+    constexpr int smem_pair = PairCfg<32>::STAGES * PairCfg<32>::STAGE_BYTES + 1024 + 256 + kGatedStageBytes;
+    static bool configured[kMaxDevices] = {};
+    int dev = 0;
+    KAI_CUDA(cudaGetDevice(&dev));
+    if (dev < kMaxDevices && !configured[dev]) {
+        KAI_CUDA(cudaFuncSetAttribute(gemm_3xtf32_gated_kernel<256, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        KAI_CUDA(cudaFuncSetAttribute(gemm_3xtf32_gated_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_pair));
+        configured[dev] = true;
+    }
+    if (pair) {
+        gemm_3xtf32_gated_pair_kernel<<<grid, kThreads, smem_pair, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p);
+        count_tc_pair_launch();
+    } else {
+        gemm_3xtf32_gated_kernel<256, 16><<<grid, kThreads, smem, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p);
+    }
+    count_launch();
+    count_tc_launch();
+    return check_launch("gemm_3xtf32_gated_kernel");
+}
+
 // Launches the GEMM kernel (and the fix-up of range-split tiles) on ready-made K-major planes
 // [rows][kp]; `partial` holds pl.slots tiles of BM x bn floats.
 static int run_tc(DeviceState* st, const TcPlan& pl, float* c, const float* a_hi, const float* a_lo,
                   const float* b_hi, const float* b_lo, int64_t M, int64_t N, int64_t K, int64_t kp, int64_t ldc,
-                  const Epilogue& ep, float* partial, int* status_dev, cudaStream_t s, bool mixed = false) {
-    CUtensorMap maps[4];
+                  const Epilogue& ep, float* partial, int* status_dev, cudaStream_t s, bool mixed = false,
+                  const GatedOut* gated = nullptr, float* c2 = nullptr, int64_t c_split = 0) {
+    CUtensorMap maps[6];
+    const int b_rows = (pl.pair || gated) ? pl.bn / 2 : pl.bn;
     KAI_TRY(make_map(&maps[0], a_hi, M, K, kp, BM, pl.bk));
     KAI_TRY(make_map(&maps[1], a_lo, M, K, kp, BM, pl.bk));
-    KAI_TRY(make_map(&maps[2], b_hi, N, K, kp, pl.pair ? pl.bn / 2 : pl.bn, pl.bk));
-    KAI_TRY(make_map(&maps[3], b_lo, N, K, kp, pl.pair ? pl.bn / 2 : pl.bn, pl.bk));
+    KAI_TRY(make_map(&maps[2], b_hi, N, K, kp, b_rows, pl.bk));
+    KAI_TRY(make_map(&maps[3], b_lo, N, K, kp, b_rows, pl.bk));
+    if (gated) {
+        KAI_TRY(make_map(&maps[4], gated->u_hi, N, K, kp, b_rows, pl.bk));
+        KAI_TRY(make_map(&maps[5], gated->u_lo, N, K, kp, b_rows, pl.bk));
+    }
 
     TcParams p;
     p.M = M; p.N = N; p.K = K; p.ldc = ldc; p.c = c;
@@ -1234,11 +1609,15 @@ static int run_tc(DeviceState* st, const TcPlan& pl, float* c, const float* a_hi
     p.partial = partial;
     p.status = status_dev;
     p.mixed = mixed ? 1 : 0;
+    p.c2 = c2;
+    p.c_split = c_split;
+    if (gated) { p.save_g = gated->g; p.save_u = gated->u; p.bias_u = gated->bias_u; }
 
     int rc;
     {
         ProfSpan span(0, s);
-        if (pl.pair) rc = (pl.bk == 16) ? launch_gemm_pair<16>(maps, p, pl.grid, s) : launch_gemm_pair<32>(maps, p, pl.grid, s);
+        if (gated) rc = launch_gemm_gated(maps, p, pl.pair, pl.grid, s);
+        else if (pl.pair) rc = (pl.bk == 16) ? launch_gemm_pair<16>(maps, p, pl.grid, s) : launch_gemm_pair<32>(maps, p, pl.grid, s);
         else if (pl.bn == 256 && pl.bk == 16) rc = launch_gemm<256, 16>(maps, p, pl.grid, s);
         else if (pl.bn == 256 && pl.bk == 32) rc = launch_gemm<256, 32>(maps, p, pl.grid, s);
         else if (pl.bn == 128 && pl.bk == 16) rc = launch_gemm<128, 16>(maps, p, pl.grid, s);
@@ -1249,7 +1628,8 @@ static int run_tc(DeviceState* st, const TcPlan& pl, float* c, const float* a_hi
     if (pl.sk_tiles > 0) {
         ProfSpan span(2, s);
         const dim3 fgrid(static_cast<unsigned>(pl.sk_tiles), FIXUP_PARTS);
-        if (pl.bn == 256) fixup_kernel<256><<<fgrid, 256, 0, s>>>(p);
+        if (gated) fixup_gated_kernel<<<fgrid, 256, 0, s>>>(p);
+        else if (pl.bn == 256) fixup_kernel<256><<<fgrid, 256, 0, s>>>(p);
         else if (pl.bn == 192) fixup_kernel<192><<<fgrid, 256, 0, s>>>(p);
         else fixup_kernel<128><<<fgrid, 256, 0, s>>>(p);
         count_launch();
@@ -1454,6 +1834,115 @@ int gemm_tc(DeviceState* st, int device, int layout, float* c, const float* a, c
     const float* pb_hi = b_prep ? b_prep->hi : (raw_b ? b : b_hi);
     const float* pb_lo = b_prep ? b_prep->lo : (b_lo_given ? b_lo_given : b_lo);
     KAI_TRY(run_tc(st, pl, c, pa_hi, pa_lo, pb_hi, pb_lo, M, N, K, kp, ldc, ep, partial, st->status_dev, s, mixed));
+    if (st->status_host[0] != 0)
+        return fail(KAI_E_DEVICE_WAIT, "a device-side wait ran out earlier (where=%d)", st->status_host[1]);
+    return KAI_OK;
+}
+
+// ---- gated layer ---------------------------------------------------------------------------
+// Bytes taken one after the other from the front of the workspace.
+struct Carve {
+    int64_t used = 0;
+    int64_t take(int64_t bytes) { const int64_t at = used; used += round_up(bytes, 256); return at; }
+};
+
+int gated_forward_tc(DeviceState* st, int device, float* h, float* g, float* u, const float* wg, const float* wu, const float* x,
+                     const float* bg, const float* bu, int64_t F, int64_t M, int64_t K, int act, const float* leaky_alpha,
+                     cudaStream_t s) {
+    constexpr int UNITS = 128;                       // hidden units of a tile
+    TcPlan pl;
+    KAI_TRY(plan_tc(st, M, (F + UNITS - 1) / UNITS * 2 * UNITS, K, &pl, 0, true));
+    const int64_t kp = round_up(K, 4);
+    const bool mixed = options().tc_cross_bf16.load() != 0 && K >= kCrossMinK && (K & 7) == 0;
+    // A weight whose rows TMA can read serves as its own hi plane where its split is a visible share of the call (as in
+    // gemm_tc; not in the mixed scheme, whose cross terms want rounded hi parts on the right side).
+    const bool raw = options().tc_raw_hi.load() != 2 && !mixed && (K & 3) == 0 && M <= 2048 &&
+                     ((reinterpret_cast<uintptr_t>(wg) | reinterpret_cast<uintptr_t>(wu)) & 15) == 0;
+    Carve ws;
+    const int64_t xh = ws.take(M * kp * 4), xl = ws.take(M * kp * 4);
+    const int64_t gh = raw ? 0 : ws.take(F * kp * 4), gl = ws.take(F * kp * 4);
+    const int64_t uh = raw ? 0 : ws.take(F * kp * 4), ul = ws.take(F * kp * 4);
+    const int64_t part = ws.take(pl.slots * BM * pl.bn * 4);
+    KAI_TRY(ensure_workspace(st, device, ws.used));
+    auto at = [&](int64_t off) { return reinterpret_cast<float*>(static_cast<uint8_t*>(st->ws) + off); };
+    auto aligned = [&](const float* v) { return (reinterpret_cast<uintptr_t>(v) & 15) == 0 && (K & 3) == 0 ? 1 : 0; };
+    RowJobs jobs = {{x, wg, wu}, {at(xh), raw ? nullptr : at(gh), raw ? nullptr : at(uh)}, {at(xl), at(gl), at(ul)}, {M, F, F}, K, kp,
+                    {aligned(x), aligned(wg), aligned(wu)}, {mixed ? 1 : 0, mixed ? 2 : 0, mixed ? 2 : 0}};
+    {
+        ProfSpan span(1, s);
+        int64_t blocks = ((M > F ? M : F) * (kp >> 2) + 255) / 256;
+        const int64_t cap = static_cast<int64_t>(st->sm_count) * 16;
+        if (blocks > cap) blocks = cap;
+        split_row_jobs_kernel<<<dim3(static_cast<unsigned>(blocks), 3), 256, 0, s>>>(jobs);
+        count_launch();
+        KAI_TRY(check_launch("split_row_jobs_kernel"));
+    }
+    const GatedOut out{raw ? wu : at(uh), at(ul), g, u, bu};
+    const Epilogue ep{bg, leaky_alpha, act, 0};
+    KAI_TRY(run_tc(st, pl, h, at(xh), at(xl), raw ? wg : at(gh), at(gl), M, F, K, kp, F, ep, at(part), st->status_dev, s, mixed, &out));
+    if (st->status_host[0] != 0)
+        return fail(KAI_E_DEVICE_WAIT, "a device-side wait ran out earlier (where=%d)", st->status_host[1]);
+    return KAI_OK;
+}
+
+int gated_backward_tc(DeviceState* st, int device, float* gx, float* gwg, float* gwu, float* gg, float* gu, const float* gh,
+                      const float* g, const float* u, const float* wg, const float* wu, const float* x, int64_t F, int64_t M,
+                      int64_t K, int act, const float* leaky_alpha, int acc_x, int acc_w, cudaStream_t s) {
+    BackParams p{};
+    p.gh = gh; p.g = g; p.u = u; p.wg = wg; p.wu = wu; p.x = x; p.leaky_alpha = leaky_alpha;
+    p.gg = gg; p.gu = gu;
+    p.ndat = M; p.xvec = K; p.yvec = F;
+    p.fp = round_up(F, 8);                     // each half of the pgx reduction in whole K steps
+    p.mp = round_up(M, 4);
+    p.act = act;
+    const bool cross = options().tc_cross_bf16.load() != 0;
+    p.mixed_x = cross && 2 * p.fp >= kCrossMinK;
+    p.mixed_w = cross && M >= kCrossMinK && (M & 7) == 0;
+    TcPlan px{}, pw{};
+    Carve ws;
+    int64_t dh = 0, dl = 0, wh = 0, wl = 0, th = 0, tl = 0, xh = 0, xl = 0;
+    if (gx) {
+        KAI_TRY(plan_tc(st, M, K, 2 * p.fp, &px));
+        dh = ws.take(M * 2 * p.fp * 4); dl = ws.take(M * 2 * p.fp * 4);
+        wh = ws.take(K * 2 * p.fp * 4); wl = ws.take(K * 2 * p.fp * 4);
+    }
+    if (gwg) {
+        KAI_TRY(plan_tc(st, 2 * F, K, M, &pw));
+        th = ws.take(2 * F * p.mp * 4); tl = ws.take(2 * F * p.mp * 4);
+        xh = ws.take(K * p.mp * 4); xl = ws.take(K * p.mp * 4);
+    }
+    const int64_t slots_x = px.slots * BM * px.bn * 4, slots_w = pw.slots * BM * pw.bn * 4;
+    const int64_t part = ws.take(slots_x > slots_w ? slots_x : slots_w);      // the two products follow each other
+    KAI_TRY(ensure_workspace(st, device, ws.used));
+    auto at = [&](int64_t off) { return reinterpret_cast<float*>(static_cast<uint8_t*>(st->ws) + off); };
+    if (gx) { p.d_hi = at(dh); p.d_lo = at(dl); p.w_hi = at(wh); p.w_lo = at(wl); }
+    if (gwg) { p.dt_hi = at(th); p.dt_lo = at(tl); p.xt_hi = at(xh); p.xt_lo = at(xl); }
+    uintptr_t all = 0;
+    for (const float* v : {gh, g, u, wg, wu, x, static_cast<const float*>(gg), static_cast<const float*>(gu)})
+        all |= reinterpret_cast<uintptr_t>(v);
+    p.vec = (all & 15) == 0 && (F & 3) == 0 && (K & 3) == 0;
+    const int64_t m_tiles = (M + 63) / 64;
+    const int64_t f_tiles = (p.fp + 63) / 64, k_tiles = (K + 63) / 64;
+    const int64_t d_tiles = m_tiles * f_tiles, w_tiles = gx ? f_tiles * k_tiles : 0, x_tiles = gwg ? m_tiles * k_tiles : 0;
+    if (d_tiles + 2 * w_tiles + x_tiles >= (int64_t(1) << 31)) return fail(KAI_E_TOO_LARGE, "gated_linear_backward: too many tiles");
+    p.f_tiles = static_cast<int>(f_tiles); p.k_tiles = static_cast<int>(k_tiles);
+    p.d_tiles = static_cast<int>(d_tiles); p.w_tiles = static_cast<int>(w_tiles);
+    {
+        ProfSpan span(1, s);
+        gated_backward_planes_kernel<<<static_cast<unsigned>(d_tiles + 2 * w_tiles + x_tiles), 256, 0, s>>>(p);
+        count_launch();
+        KAI_TRY(check_launch("gated_backward_planes_kernel"));
+    }
+    if (gx) {
+        const Epilogue ep{nullptr, nullptr, KAI_ACT_NONE, acc_x ? 1 : 0};
+        KAI_TRY(run_tc(st, px, gx, p.d_hi, p.d_lo, p.w_hi, p.w_lo, M, K, 2 * p.fp, 2 * p.fp, K, ep, at(part), st->status_dev, s,
+                       p.mixed_x != 0));
+    }
+    if (gwg) {
+        const Epilogue ep{nullptr, nullptr, KAI_ACT_NONE, acc_w ? 1 : 0};
+        KAI_TRY(run_tc(st, pw, gwg, p.dt_hi, p.dt_lo, p.xt_hi, p.xt_lo, 2 * F, K, M, p.mp, K, ep, at(part), st->status_dev, s,
+                       p.mixed_w != 0, nullptr, gwu, F));
+    }
     if (st->status_host[0] != 0)
         return fail(KAI_E_DEVICE_WAIT, "a device-side wait ran out earlier (where=%d)", st->status_host[1]);
     return KAI_OK;
