@@ -57,6 +57,9 @@ int gated_forward_tc(DeviceState*, int, float*, float*, float*, const float*, co
 int gated_backward_tc(DeviceState*, int, float*, float*, float*, float*, float*, const float*, const float*, const float*,
                       const float*, const float*, const float*, int64_t, int64_t, int64_t, int, const float*, int, int,
                       cudaStream_t);
+bool gated_skinny_takes(int64_t, int64_t, const float*, const float*, const float*);
+int gated_skinny(DeviceState*, float*, float*, float*, const float*, const float*, const float*, const float*, const float*,
+                 int64_t, int64_t, int64_t, int, const float*, cudaStream_t);
 int gated_forward_mma(DeviceState*, float*, float*, float*, const float*, const float*, const float*, const float*, const float*,
                       int64_t, int64_t, int64_t, int, const float*, cudaStream_t);
 int gated_backward_mma(DeviceState*, float*, float*, float*, const float*, const float*, const float*, const float*,
@@ -491,6 +494,9 @@ int kai_set_option(const char* name, int64_t value) {
     } else if (!strcmp(name, "gated_tc_flops")) {
         if (value < 0) return fail(KAI_E_INVALID_ARG, "gated_tc_flops must be >= 0");
         o.gated_tc_flops = value;
+    } else if (!strcmp(name, "gated_raw_rows")) {
+        if (value < 0) return fail(KAI_E_INVALID_ARG, "gated_raw_rows must be >= 0");
+        o.gated_raw_rows = value;
     } else if (!strcmp(name, "split_k")) {
         if (value < 0 || value > 64) return fail(KAI_E_INVALID_ARG, "split_k must be in 0..64");
         o.split_k = value;
@@ -556,6 +562,7 @@ int64_t kai_get_option(const char* name) {
     if (!strcmp(name, "tc_bk")) return o.tc_bk;
     if (!strcmp(name, "tc_min_flops")) return o.tc_min_flops;
     if (!strcmp(name, "gated_tc_flops")) return o.gated_tc_flops;
+    if (!strcmp(name, "gated_raw_rows")) return o.gated_raw_rows;
     if (!strcmp(name, "split_k")) return o.split_k;
     if (!strcmp(name, "path")) return o.path;
     if (!strcmp(name, "tc_group_m")) return o.tc_group_m;
@@ -1477,6 +1484,8 @@ int kai_gated_linear_forward(int device, float* ph, float* pg, float* pu, const 
     KAI_ENTER(device);
     if (ndat == 0 || yvec == 0) return KAI_OK;
     const double flops = 4.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
+    if (gated_skinny_takes(ndat, xvec, px, pwg, pwu))
+        return gated_skinny(st, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
     if (xvec > 0 && ndat > 16 && flops >= static_cast<double>(options().gated_tc_flops.load()))
         return gated_forward_tc(st, device, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
     return gated_forward_mma(st, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
@@ -1505,7 +1514,7 @@ int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float* pgwu, 
     }
     if (clash) return fail(KAI_E_INVALID_ARG, "gated_linear_backward: two buffers overlap");
     KAI_ENTER(device);
-    const double flops = 8.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
+    const double flops = 4.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
     if (ndat > 16 && flops > 0.0 && flops >= static_cast<double>(options().gated_tc_flops.load()) && (pgx || pgwg))
         return gated_backward_tc(st, device, pgx, pgwg, pgwu, pgg, pgu, pgh, pg, pu, pwg, pwu, px, yvec, ndat, xvec, act,
                                  leaky_alpha, acc_x, acc_w, s);

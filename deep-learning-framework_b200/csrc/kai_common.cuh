@@ -38,7 +38,8 @@ struct Options {
     std::atomic<int64_t> tc_bn{256};
     std::atomic<int64_t> tc_bk{16};
     std::atomic<int64_t> tc_min_flops{int64_t(1) << 29};  // below: SIMT kernel
-    std::atomic<int64_t> gated_tc_flops{int64_t(1) << 26};  // gated layer: tensor-core kernels from here on
+    std::atomic<int64_t> gated_tc_flops{1200000000};        // gated layer: flops of its forward products from which on the tensor-core GEMM takes them
+    std::atomic<int64_t> gated_raw_rows{384};             // gated layer: most rows whose forward call works without operand planes
     std::atomic<int64_t> split_k{0};                      // 0 = automatic
     std::atomic<int64_t> path{KAI_PATH_AUTO};
     std::atomic<int64_t> tc_group_m{16};                  // rasterisation group (tiles along M)

@@ -68,21 +68,37 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
+// What the gated form needs beside the plain one: the second weight and where the factors go.  A tile of 16 rows is then 8 rows of
+// the gate weight and the 8 rows of the up weight for the same hidden units.
+struct SkinnyGate {
+    const float* wu;
+    const float* bias_u;
+    float* g;
+    float* u;
+};
+__device__ __forceinline__ void store_gate(const SkinnyGate& gate, float* y, int64_t at, int64_t n, float g, float u,
+                                           const float* __restrict__ bias, int act, float alpha) {
+    if (bias) g += __ldg(bias + n);
+    if (gate.bias_u) u += __ldg(gate.bias_u + n);
+    if (gate.g) { gate.g[at] = g; gate.u[at] = u; }
+    y[at] = act_forward(act, g, alpha) * u;
+}
+
 // NT = number of 8-column output tiles: 1 for M <= 8, 2 for M <= 16.
-template <int NT>
+template <int NT, bool GATED = false>
 __global__ void __launch_bounds__(SKM_WARPS * 32, 2)
 skinny_mma_kernel(const float* __restrict__ x, const float* __restrict__ w, float* __restrict__ y, int M, int64_t N,
                   int64_t K, int64_t ldc, int64_t k_per_warp, const float* __restrict__ bias,
-                  const float* __restrict__ leaky_alpha, int act, int accumulate) {
+                  const float* __restrict__ leaky_alpha, int act, int accumulate, const SkinnyGate gate) {
     __shared__ float red[SKM_WARPS][16][8 * NT + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (GATED ? 8 : 16);
     // rows past N are clamped (their results are never stored)
     const int64_t r0 = (n0 + g < N) ? (n0 + g) : (N - 1);
-    const int64_t r1 = (n0 + g + 8 < N) ? (n0 + g + 8) : (N - 1);
+    const int64_t r1 = GATED ? r0 : (n0 + g + 8 < N) ? (n0 + g + 8) : (N - 1);
     const float* w0 = w + r0 * K + 4 * t;
-    const float* w1 = w + r1 * K + 4 * t;
+    const float* w1 = (GATED ? gate.wu : w) + r1 * K + 4 * t;
     const float* xrow[NT];
     bool xvalid[NT];
 #pragma unroll
@@ -190,6 +206,18 @@ skinny_mma_kernel(const float* __restrict__ x, const float* __restrict__ w, floa
     __syncthreads();
 
     const float alpha = (leaky_alpha != nullptr) ? __ldg(leaky_alpha) : 0.0f;
+    if (GATED) {
+        for (int e = threadIdx.x; e < 8 * 8 * NT; e += SKM_WARPS * 32) {
+            const int r = e & 7, m = e >> 3;
+            const int64_t n = n0 + r;
+            if (n >= N || m >= M) continue;
+            float sg = 0.0f, su = 0.0f;
+#pragma unroll
+            for (int ww = 0; ww < SKM_WARPS; ++ww) { sg += red[ww][r][m]; su += red[ww][r + 8][m]; }
+            store_gate(gate, y, static_cast<int64_t>(m) * ldc + n, n, sg, su, bias, act, alpha);
+        }
+        return;
+    }
     for (int e = threadIdx.x; e < 16 * 8 * NT; e += SKM_WARPS * 32) {
         const int r = e & 15, m = e >> 4;      // consecutive threads -> consecutive columns of Y
         const int64_t n = n0 + r;
@@ -210,15 +238,17 @@ skinny_mma_kernel(const float* __restrict__ x, const float* __restrict__ w, floa
 // block's rows of W, 2 KB contiguous per row -- one DRAM page, asked for at once -- two rows per step of the same
 // per-lane cp.async ring.  Per row a shuffle tree adds the lanes; the eight warps (eight ranges of K) add up through
 // shared memory in warp order at the end.
-constexpr int SKF_ROWS = 16;       // most rows of W a block takes
+constexpr int SKF_ROWS = 16;       // most rows of W a block takes (gated: hidden units, two rows each)
 constexpr int SKF_KW = 512;        // values of K per warp: 4 pieces x 32 lanes x 4 floats
 
-template <int MF>
+// GATED: the two rows of a step are the gate's and the up projection's of one hidden unit; N and rows_per_block count units.
+template <int MF, bool GATED = false>
 __global__ void __launch_bounds__(SKM_WARPS * 32, 2)
 skinny_fma_kernel(const float* __restrict__ x, const float* __restrict__ w, float* __restrict__ y, int M, int64_t N,
                   int64_t K, int64_t ldc, int rows_per_block, const float* __restrict__ bias,
-                  const float* __restrict__ leaky_alpha, int act, int accumulate) {
-    __shared__ float red[SKM_WARPS][SKF_ROWS][MF];
+                  const float* __restrict__ leaky_alpha, int act, int accumulate, const SkinnyGate gate) {
+    constexpr int ROWS = GATED ? 2 * SKF_ROWS : SKF_ROWS;
+    __shared__ float red[SKM_WARPS][ROWS][MF];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
     const int nrows = static_cast<int>((N - r0 < rows_per_block) ? (N - r0) : rows_per_block);
@@ -234,15 +264,16 @@ skinny_fma_kernel(const float* __restrict__ x, const float* __restrict__ w, floa
 
     extern __shared__ float4 skm_ring[];          // [warp][stage][piece 0..7][lane]; pieces 0-3 = first row of the step
     float4* ring = skm_ring + static_cast<size_t>(warp) * SKM_STAGES * 8 * 32 + lane;
-    const int steps = (nrows + 1) >> 1;
+    const int steps = GATED ? nrows : (nrows + 1) >> 1;
     auto issue = [&](int step, int stage) {
         float4* dst = ring + stage * 8 * 32;
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-            const int row = 2 * step + (p >> 2);
+            const int row = GATED ? step : 2 * step + (p >> 2);
             const int64_t k = kb + 128 * (p & 3);
             const bool in = step < steps && row < nrows && k < K;
-            cp_async16(dst + p * 32, in ? (w + (r0 + row) * K + k) : w, in);
+            const float* from = (GATED && (p >> 2)) ? gate.wu : w;
+            cp_async16(dst + p * 32, in ? (from + (r0 + row) * K + k) : w, in);
         }
         cp_async_commit();                          // one group per step, also when it is empty
     };
@@ -269,7 +300,7 @@ skinny_fma_kernel(const float* __restrict__ x, const float* __restrict__ w, floa
                     v = fmaf(wv[i].w, xr[m][i].w, fmaf(wv[i].z, xr[m][i].z, fmaf(wv[i].y, xr[m][i].y, fmaf(wv[i].x, xr[m][i].x, v))));
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                if (lane == 0 && 2 * step + rr < SKF_ROWS) red[warp][2 * step + rr][m] = v;
+                if (lane == 0 && 2 * step + rr < ROWS) red[warp][2 * step + rr][m] = v;
             }
         }
         if (++stage == SKM_STAGES) stage = 0;
@@ -279,6 +310,13 @@ skinny_fma_kernel(const float* __restrict__ x, const float* __restrict__ w, floa
     for (int e = threadIdx.x; e < SKF_ROWS * MF; e += SKM_WARPS * 32) {
         const int r = e % SKF_ROWS, m = e / SKF_ROWS;      // consecutive threads -> consecutive columns of Y
         if (r >= nrows || m >= M) continue;
+        if (GATED) {
+            float sg = 0.0f, su = 0.0f;
+#pragma unroll
+            for (int ww = 0; ww < SKM_WARPS; ++ww) { sg += red[ww][2 * r][m]; su += red[ww][2 * r + 1][m]; }
+            store_gate(gate, y, static_cast<int64_t>(m) * ldc + r0 + r, r0 + r, sg, su, bias, act, alpha);
+            continue;
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int ww = 0; ww < SKM_WARPS; ++ww) sum += red[ww][r][m];
@@ -312,7 +350,7 @@ int gemm_skinny_mma(float* c, const float* x, const float* w, int64_t M, int64_t
         KAI_CUDA(cudaFuncSetAttribute(skinny_fma_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
         configured[dev] = true;
     }
-#define KAI_SKM_ARGS x, w, c, static_cast<int>(M), N, K, ldc, k_per_warp, ep.bias, ep.leaky_alpha, ep.act, ep.accumulate
+#define KAI_SKM_ARGS x, w, c, static_cast<int>(M), N, K, ldc, k_per_warp, ep.bias, ep.leaky_alpha, ep.act, ep.accumulate, SkinnyGate{}
     if (M <= 4 && K <= SKM_WARPS * SKF_KW) {
         // Rows per block (even, at most 16) chosen so that the blocks fill two per SM evenly: 4096 rows on 148 SMs are
         // 14 rows x 293 blocks, where 16 rows x 256 blocks would leave 40 SMs with half the work of the others.
@@ -323,7 +361,7 @@ int gemm_skinny_mma(float* c, const float* x, const float* w, int64_t M, int64_t
         if (rpb > SKF_ROWS) rpb = SKF_ROWS;
         if (rpb < 2) rpb = 2;
         const unsigned fgrid = static_cast<unsigned>((N + rpb - 1) / rpb);
-#define KAI_SKF_ARGS x, w, c, static_cast<int>(M), N, K, ldc, static_cast<int>(rpb), ep.bias, ep.leaky_alpha, ep.act, ep.accumulate
+#define KAI_SKF_ARGS x, w, c, static_cast<int>(M), N, K, ldc, static_cast<int>(rpb), ep.bias, ep.leaky_alpha, ep.act, ep.accumulate, SkinnyGate{}
         if (M == 1) skinny_fma_kernel<1><<<fgrid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKF_ARGS);
         else if (M == 2) skinny_fma_kernel<2><<<fgrid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKF_ARGS);
         else skinny_fma_kernel<4><<<fgrid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKF_ARGS);
@@ -334,6 +372,47 @@ int gemm_skinny_mma(float* c, const float* x, const float* w, int64_t M, int64_t
 #undef KAI_SKM_ARGS
     count_launch();
     return check_launch("skinny_mma_kernel");
+}
+
+// The gated layer for a handful of rows: both weights streamed once, h = act(g) * u in the same launch.
+bool gated_skinny_takes(int64_t M, int64_t K, const float* x, const float* wg, const float* wu) {
+    return M >= 1 && M <= 16 && K >= 64 && (K & 3) == 0 &&
+           ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(wg) | reinterpret_cast<uintptr_t>(wu)) & 15) == 0;
+}
+int gated_skinny(DeviceState* st, float* h, float* g, float* u, const float* wg, const float* wu, const float* x, const float* bg,
+                 const float* bu, int64_t F, int64_t M, int64_t K, int act, const float* leaky_alpha, cudaStream_t s) {
+    static bool configured[kMaxDevices] = {};
+    int dev = 0;
+    KAI_CUDA(cudaGetDevice(&dev));
+    if (dev < kMaxDevices && !configured[dev]) {
+        KAI_CUDA(cudaFuncSetAttribute(skinny_mma_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
+        KAI_CUDA(cudaFuncSetAttribute(skinny_mma_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
+        KAI_CUDA(cudaFuncSetAttribute(skinny_fma_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
+        KAI_CUDA(cudaFuncSetAttribute(skinny_fma_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
+        KAI_CUDA(cudaFuncSetAttribute(skinny_fma_kernel<4, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
+        configured[dev] = true;
+    }
+    const SkinnyGate gate{wu, bu, g, u};
+    const int m = static_cast<int>(M);
+    if (M <= 4 && K <= SKM_WARPS * SKF_KW) {
+        // units per block so that the blocks fill two per SM evenly, as above
+        int64_t units = (F + 2 * static_cast<int64_t>(st->sm_count) - 1) / (2 * static_cast<int64_t>(st->sm_count));
+        if (units > SKF_ROWS) units = SKF_ROWS;
+        const unsigned grid = static_cast<unsigned>((F + units - 1) / units);
+#define KAI_SKG_ARGS x, wg, h, m, F, K, F, static_cast<int>(units), bg, leaky_alpha, act, 0, gate
+        if (M == 1) skinny_fma_kernel<1, true><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
+        else if (M == 2) skinny_fma_kernel<2, true><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
+        else skinny_fma_kernel<4, true><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
+#undef KAI_SKG_ARGS
+    } else {
+        const unsigned grid = static_cast<unsigned>((F + 7) / 8);
+#define KAI_SKG_ARGS x, wg, h, m, F, K, F, int64_t(0), bg, leaky_alpha, act, 0, gate
+        if (M <= 8) skinny_mma_kernel<1, true><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
+        else skinny_mma_kernel<2, true><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
+#undef KAI_SKG_ARGS
+    }
+    count_launch();
+    return check_launch("gated skinny kernel");
 }
 
 }  // namespace kai

@@ -196,6 +196,7 @@ __device__ __forceinline__ void store_chunk(const TcParams& p, const WorkItem& i
                                             int col_in_tile, const float* r, bool vec_ok, float alpha) {
     if (it.slot >= 0) {
         // Piece of a range-split tile: raw sums, tile-local layout, always 16-byte aligned.
+        if (static_cast<int64_t>(it.m_blk) * BM + row_in_tile >= p.M) return;
         float* out = p.partial + (static_cast<int64_t>(it.slot) * BM + row_in_tile) * BN + col_in_tile;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -333,36 +334,74 @@ __device__ __forceinline__ void store_half(const TcParams& p, const WorkItem& it
     }
 }
 
+// Lo tile of a raw fp32 tile, at the same offsets: the part below the 11 bits that the tensor core reads, rounded to 11 bits of
+// its own.  All threads of the epilogue warps together.
+template <int BYTES>
+__device__ __forceinline__ void split_tile(const uint8_t* raw, uint8_t* lo, int bytes) {
+    constexpr int N = BYTES / 16, T = 32 * kEpiWarps;
+    static_assert(N % T == 0, "whole pieces per thread");
+#pragma unroll
+    for (int i = 0; i < N / T; ++i) {
+        const int at = (static_cast<int>(threadIdx.x) - 64 + i * T) * 16;
+        if (at >= bytes) break;
+        float4 v = *reinterpret_cast<const float4*>(raw + at);
+        float* f = reinterpret_cast<float*>(&v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float rest = f[e] - __uint_as_float(__float_as_uint(f[e]) & 0xFFFFE000u);
+            f[e] = isfinite(f[e]) ? __uint_as_float(__float_as_uint(rest) + 0x1000u) : 0.0f;
+        }
+        *reinterpret_cast<float4*>(lo + at) = v;
+    }
+}
+
 // ---------------------------------------------------------------------------------------
 // The GEMM kernel
 // ---------------------------------------------------------------------------------------
 // GATED: the B tile's first BN / 2 rows come from map_b_* (gate weights), the others from map_u_* (up weights), at the
 // same hidden units.
-template <int BN, int BK, int KH, bool GATED = false>
+//
+// RAW: both operands are fp32 matrices as they are; the producer fetches one box of each per stage, which serves as hi plane (the
+// tensor core ignores the low 13 mantissa bits), and the epilogue warps derive the lo tiles, element for element at the
+// same swizzled offset, before they hand the block to the MMA thread.  The fp32 boxes have a ring of six stages of 24 KB -- the stream
+// of weights is what the kernel waits for -- and the lo tiles one of two.  The epilogue warps promote a chunk's sums one chunk
+// late, so that conversions never wait for the MMAs that they feed.
+template <int BN, int BK, int KH, bool GATED = false, bool RAW = false>
 __device__ __forceinline__ void
 gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const CUtensorMap& map_b_hi,
                  const CUtensorMap& map_b_lo, const TapMaps* taps, const TcParams& p, const CUtensorMap* map_u_hi = nullptr,
                  const CUtensorMap* map_u_lo = nullptr) {
     using C = Cfg<BN, BK>;
+    constexpr int STAGES = RAW ? 196608 / C::STAGE_BYTES * 3 / 2 : C::STAGES;
+    constexpr int STAGE_BYTES = RAW ? C::STAGE_BYTES / 2 : C::STAGE_BYTES;
+    constexpr int LO_STAGES = 2;                          // RAW: lo tiles behind the ring
+    static_assert(!RAW || STAGES * STAGE_BYTES + LO_STAGES * STAGE_BYTES <= 196608, "both rings in the shared memory of one");
     extern __shared__ uint8_t smem_raw[];
     // Swizzled tiles need their base on a 1024-byte boundary.
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
     uint64_t* full_bar = bars;                       // [STAGES]  TMA -> MMA
-    uint64_t* empty_bar = bars + C::STAGES;          // [STAGES]  MMA -> TMA
-    uint64_t* tmem_full_bar = bars + 2 * C::STAGES;  // [2]       MMA -> epilogue
+    uint64_t* empty_bar = bars + STAGES;          // [STAGES]  MMA -> TMA
+    uint64_t* tmem_full_bar = bars + 2 * STAGES;  // [2]       MMA -> epilogue
     uint64_t* tmem_empty_bar = tmem_full_bar + 2;    // [2]       epilogue -> MMA
     uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty_bar + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
+    uint64_t* split_bar = reinterpret_cast<uint64_t*>(tmem_base_slot + 2);   // [LO_STAGES]  RAW: epilogue warps -> MMA
+    uint64_t* lo_empty_bar = split_bar + LO_STAGES;                          // [LO_STAGES]  RAW: MMA -> epilogue warps
+    uint8_t* lo_tiles = smem + STAGES * STAGE_BYTES;
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < C::STAGES; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&full_bar[s]), 1);
             mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        for (int s = 0; RAW && s < LO_STAGES; ++s) {
+            mbar_init(smem_u32(&split_bar[s]), kEpiWarps);
+            mbar_init(smem_u32(&lo_empty_bar[s]), 1);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(smem_u32(&tmem_full_bar[s]), 1);
@@ -410,12 +449,17 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
                     ok = mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag, p.status, 1);
                     if (!ok) break;
                     const uint32_t full = smem_u32(&full_bar[stage]);
-                    uint8_t* base = smem + stage * C::STAGE_BYTES;
-                    mbar_expect_tx(full, C::STAGE_BYTES);
+                    uint8_t* base = smem + stage * STAGE_BYTES;
+                    mbar_expect_tx(full, STAGE_BYTES);
                     const int k0 = kb * BK;
                     tma_load_2d(smem_u32(base), &map_a_hi, full, k0, row_a);
-                    tma_load_2d(smem_u32(base + C::A_BYTES), &map_a_lo, full, k0, row_a);
-                    if (GATED) {
+                    if (!RAW) tma_load_2d(smem_u32(base + C::A_BYTES), &map_a_lo, full, k0, row_a);
+                    if (RAW) {
+                        constexpr int SUB = C::B_BYTES / 2;
+                        const int unit = it.n_blk * (BN / 2);
+                        tma_load_2d(smem_u32(base + C::A_BYTES), &map_b_hi, full, k0, unit);
+                        tma_load_2d(smem_u32(base + C::A_BYTES + SUB), map_u_hi, full, k0, unit);
+                    } else if (GATED) {
                         constexpr int SUB = C::B_BYTES / 2;
                         const int unit = it.n_blk * (BN / 2);
                         tma_load_2d(smem_u32(base + 2 * C::A_BYTES), &map_b_hi, full, k0, unit);
@@ -435,7 +479,7 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
                                         chan0, shift);
                         }
                     }
-                    if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
         }
@@ -446,6 +490,8 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
             const uint32_t idesc16 = instr_desc_bf16(BM, BN);
             int stage = 0;
             uint32_t phase = 0;
+            int lo_stage = 0;
+            uint32_t lo_phase = 0;
             int acc_buf = 0;
             uint32_t acc_phase = 0;
             bool ok = true;
@@ -461,14 +507,16 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc_buf * BN);
                     for (int kb = kb0; kb < kb1; ++kb) {
-                        ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, 3);
+                        ok = RAW ? mbar_wait(smem_u32(&split_bar[lo_stage]), lo_phase, abort_flag, p.status, 3)
+                                 : mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, 3);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t base = smem_u32(smem + stage * C::STAGE_BYTES);
+                        const uint32_t base = smem_u32(smem + stage * STAGE_BYTES);
                         const uint64_t a_hi = smem_desc_kmajor<BK>(base);
-                        const uint64_t a_lo = smem_desc_kmajor<BK>(base + C::A_BYTES);
-                        const uint64_t b_hi = smem_desc_kmajor<BK>(base + 2 * C::A_BYTES);
-                        const uint64_t b_lo = smem_desc_kmajor<BK>(base + 2 * C::A_BYTES + C::B_BYTES);
+                        const uint32_t lo = smem_u32(lo_tiles + lo_stage * STAGE_BYTES);
+                        const uint64_t a_lo = smem_desc_kmajor<BK>(RAW ? lo : base + C::A_BYTES);
+                        const uint64_t b_hi = smem_desc_kmajor<BK>(RAW ? base + C::A_BYTES : base + 2 * C::A_BYTES);
+                        const uint64_t b_lo = smem_desc_kmajor<BK>(RAW ? lo + C::A_BYTES : base + 2 * C::A_BYTES + C::B_BYTES);
 #pragma unroll
                         for (int k = 0; k < BK / UMMA_K; ++k) {
                             // Advancing inside the swizzle span: +32 bytes = +2 in the (addr >> 4) field.
@@ -484,7 +532,11 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
                             umma_tf32(d_tmem, a_hi + adv, b_hi + adv, idesc, 1u);
                         }
                         umma_commit(smem_u32(&empty_bar[stage]));  // slot reusable once these MMAs retire
-                        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                        if (RAW) {
+                            umma_commit(smem_u32(&lo_empty_bar[lo_stage]));
+                            if (++lo_stage == LO_STAGES) { lo_stage = 0; lo_phase ^= 1u; }
+                        }
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
                     if (!ok) break;
                     umma_commit(smem_u32(&tmem_full_bar[acc_buf]));  // chunk complete
@@ -504,13 +556,38 @@ gemm_3xtf32_body(const CUtensorMap& map_a_hi, const CUtensorMap& map_a_lo, const
         const bool vec_ok = (p.ldc & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.c) | reinterpret_cast<uintptr_t>(p.c2)) & 15) == 0;
         int acc_buf = 0;
         uint32_t acc_phase = 0;
+        int stage = 0, lo_stage = 0;
+        uint32_t phase = 0, lo_phase = 0;
         bool ok = true;
         WorkIter iter(p);
         WorkItem it;
         while (ok && iter.next(p, it)) {
             float acc[HALF];
             bool first_chunk = true;
+            int conv = it.kb_begin;            // RAW: next K block to split
+            // rows of A beyond M are not looked at: their lo tiles may hold anything
+            const int64_t a_rows = p.M - static_cast<int64_t>(it.m_blk) * BM;
+            const int a_bytes = a_rows < BM ? static_cast<int>(a_rows + 7) / 8 * 8 * BK * 4 : C::A_BYTES;
             for (int kb0 = it.kb_begin; kb0 < it.kb_end; kb0 += p.kc_blocks) {
+                if (RAW) {
+                    // the blocks of this chunk (first time) and of the next one
+                    const int upto = min(it.kb_end, kb0 + 2 * p.kc_blocks);
+                    for (; ok && conv < upto; ++conv) {
+                        ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, 9);
+                        ok = ok && mbar_wait(smem_u32(&lo_empty_bar[lo_stage]), lo_phase ^ 1u, abort_flag, p.status, 10);
+                        if (!ok) break;
+                        const uint8_t* at = smem + stage * STAGE_BYTES;
+                        uint8_t* lo = lo_tiles + lo_stage * STAGE_BYTES;
+                        split_tile<C::A_BYTES>(at, lo, a_bytes);
+                        split_tile<C::B_BYTES>(at + C::A_BYTES, lo + C::A_BYTES, C::B_BYTES);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&split_bar[lo_stage]));
+                        if (++lo_stage == LO_STAGES) { lo_stage = 0; lo_phase ^= 1u; }
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    }
+                    if (!ok) break;
+                }
                 ok = mbar_wait(smem_u32(&tmem_full_bar[acc_buf]), acc_phase, abort_flag, p.status, 4);
                 if (!ok) break;
                 tc_fence_after();
@@ -574,6 +651,14 @@ gemm_3xtf32_gated_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __g
                          const __grid_constant__ CUtensorMap map_u_hi, const __grid_constant__ CUtensorMap map_u_lo,
                          const TcParams p) {
     gemm_3xtf32_body<BN, BK, 0, true>(map_a_hi, map_a_lo, map_g_hi, map_g_lo, nullptr, p, &map_u_hi, &map_u_lo);
+}
+
+// The same from the operands as they are: for a few rows of x the weights are read once, 4 bytes per value, instead of becoming
+// planes first.
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_3xtf32_gated_raw_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_g,
+                             const __grid_constant__ CUtensorMap map_u, const TcParams p) {
+    gemm_3xtf32_body<256, 16, 0, true, true>(map_a, map_a, map_g, map_g, nullptr, p, &map_u, &map_u);
 }
 
 // The same kernel with the B operand in tap-row form (see TcParams): the kernel gradient of a convolution read
@@ -1449,7 +1534,8 @@ static int64_t max_slots(int64_t tiles, int sms, int forced) {
     return rem > 0 ? rem + sms : 0;
 }
 
-static int plan_tc(const DeviceState* st, int64_t M, int64_t N, int64_t K, TcPlan* out, int force_bn = 0, bool gated = false) {
+static int plan_tc(const DeviceState* st, int64_t M, int64_t N, int64_t K, TcPlan* out, int force_bn = 0, bool gated = false,
+                   bool no_pair = false) {
     if (M >= (int64_t(1) << 31) || N >= (int64_t(1) << 31) || K >= (int64_t(1) << 31))
         return fail(KAI_E_TOO_LARGE, "gemm_tc: a dimension exceeds 2^31-1");
     Options& opt = options();
@@ -1488,7 +1574,7 @@ static int plan_tc(const DeviceState* st, int64_t M, int64_t N, int64_t K, TcPla
 
     // The CTA-pair kernel takes the call when the 256 x 256 tiles fill at least half a round of the pairs and the
     // second half of the last tile row is not mostly padding.
-    if (opt.tc_pair.load() != 0 && pl.bn == 256 && force_bn == 0 && forced <= 0 && sms >= 2 &&
+    if (!no_pair && opt.tc_pair.load() != 0 && pl.bn == 256 && force_bn == 0 && forced <= 0 && sms >= 2 &&
         (pl.tiles_m % 2 == 0 || pl.tiles_m >= 9)) {
         const int tiles_mp = (pl.tiles_m + 1) / 2;
         const int64_t tiles_p = static_cast<int64_t>(tiles_mp) * pl.tiles_n;
@@ -1556,9 +1642,10 @@ struct GatedOut {
     float* g;
     float* u;
     const float* bias_u;
+    bool raw;            // operands as they are, no planes
 };
 
-static int launch_gemm_gated(const CUtensorMap maps[6], const TcParams& p, bool pair, int grid, cudaStream_t s) {
+static int launch_gemm_gated(const CUtensorMap maps[6], const TcParams& p, bool pair, bool raw, int grid, cudaStream_t s) {
     using C = Cfg<256, 16>;
     constexpr int smem = C::STAGES * C::STAGE_BYTES + 1024 + 256 + kGatedStageBytes;
     constexpr int smem_pair = PairCfg<32>::STAGES * PairCfg<32>::STAGE_BYTES + 1024 + 256 + kGatedStageBytes;
@@ -1567,10 +1654,13 @@ static int launch_gemm_gated(const CUtensorMap maps[6], const TcParams& p, bool 
     KAI_CUDA(cudaGetDevice(&dev));
     if (dev < kMaxDevices && !configured[dev]) {
         KAI_CUDA(cudaFuncSetAttribute(gemm_3xtf32_gated_kernel<256, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        KAI_CUDA(cudaFuncSetAttribute(gemm_3xtf32_gated_raw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         KAI_CUDA(cudaFuncSetAttribute(gemm_3xtf32_gated_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_pair));
         configured[dev] = true;
     }
-    if (pair) {
+    if (raw) {
+        gemm_3xtf32_gated_raw_kernel<<<grid, kThreads, smem, s>>>(maps[0], maps[2], maps[4], p);
+    } else if (pair) {
         gemm_3xtf32_gated_pair_kernel<<<grid, kThreads, smem_pair, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p);
         count_tc_pair_launch();
     } else {
@@ -1590,12 +1680,13 @@ static int run_tc(DeviceState* st, const TcPlan& pl, float* c, const float* a_hi
     CUtensorMap maps[6];
     const int b_rows = (pl.pair || gated) ? pl.bn / 2 : pl.bn;
     KAI_TRY(make_map(&maps[0], a_hi, M, K, kp, BM, pl.bk));
-    KAI_TRY(make_map(&maps[1], a_lo, M, K, kp, BM, pl.bk));
+    const bool planes = !(gated && gated->raw);
+    if (planes) KAI_TRY(make_map(&maps[1], a_lo, M, K, kp, BM, pl.bk));
     KAI_TRY(make_map(&maps[2], b_hi, N, K, kp, b_rows, pl.bk));
-    KAI_TRY(make_map(&maps[3], b_lo, N, K, kp, b_rows, pl.bk));
+    if (planes) KAI_TRY(make_map(&maps[3], b_lo, N, K, kp, b_rows, pl.bk));
     if (gated) {
         KAI_TRY(make_map(&maps[4], gated->u_hi, N, K, kp, b_rows, pl.bk));
-        KAI_TRY(make_map(&maps[5], gated->u_lo, N, K, kp, b_rows, pl.bk));
+        if (planes) KAI_TRY(make_map(&maps[5], gated->u_lo, N, K, kp, b_rows, pl.bk));
     }
 
     TcParams p;
@@ -1616,7 +1707,7 @@ static int run_tc(DeviceState* st, const TcPlan& pl, float* c, const float* a_hi
     int rc;
     {
         ProfSpan span(0, s);
-        if (gated) rc = launch_gemm_gated(maps, p, pl.pair, pl.grid, s);
+        if (gated) rc = launch_gemm_gated(maps, p, pl.pair, gated->raw, pl.grid, s);
         else if (pl.pair) rc = (pl.bk == 16) ? launch_gemm_pair<16>(maps, p, pl.grid, s) : launch_gemm_pair<32>(maps, p, pl.grid, s);
         else if (pl.bn == 256 && pl.bk == 16) rc = launch_gemm<256, 16>(maps, p, pl.grid, s);
         else if (pl.bn == 256 && pl.bk == 32) rc = launch_gemm<256, 32>(maps, p, pl.grid, s);
@@ -1851,8 +1942,22 @@ int gated_forward_tc(DeviceState* st, int device, float* h, float* g, float* u, 
                      cudaStream_t s) {
     constexpr int UNITS = 128;                       // hidden units of a tile
     TcPlan pl;
-    KAI_TRY(plan_tc(st, M, (F + UNITS - 1) / UNITS * 2 * UNITS, K, &pl, 0, true));
     const int64_t kp = round_up(K, 4);
+    // Without planes: rows that TMA can read, and few enough of them that the weights' traffic counts for more than the products.
+    if ((K & 3) == 0 && M <= options().gated_raw_rows.load() &&
+        ((reinterpret_cast<uintptr_t>(wg) | reinterpret_cast<uintptr_t>(wu) | reinterpret_cast<uintptr_t>(x)) & 15) == 0) {
+        KAI_TRY(plan_tc(st, M, (F + UNITS - 1) / UNITS * 2 * UNITS, K, &pl, 0, true, true));
+        const int64_t bytes = pl.slots * BM * pl.bn * 4;
+        if (bytes > 0) KAI_TRY(ensure_workspace(st, device, bytes));
+        const GatedOut out{wu, nullptr, g, u, bu, true};
+        const Epilogue ep{bg, leaky_alpha, act, 0};
+        KAI_TRY(run_tc(st, pl, h, x, nullptr, wg, nullptr, M, F, K, kp, F, ep, static_cast<float*>(st->ws), st->status_dev, s, false,
+                       &out));
+        if (st->status_host[0] != 0)
+            return fail(KAI_E_DEVICE_WAIT, "a device-side wait ran out earlier (where=%d)", st->status_host[1]);
+        return KAI_OK;
+    }
+    KAI_TRY(plan_tc(st, M, (F + UNITS - 1) / UNITS * 2 * UNITS, K, &pl, 0, true));
     const bool mixed = options().tc_cross_bf16.load() != 0 && K >= kCrossMinK && (K & 7) == 0;
     // A weight whose rows TMA can read serves as its own hi plane where its split is a visible share of the call (as in
     // gemm_tc; not in the mixed scheme, whose cross terms want rounded hi parts on the right side).
@@ -1877,7 +1982,7 @@ int gated_forward_tc(DeviceState* st, int device, float* h, float* g, float* u, 
         count_launch();
         KAI_TRY(check_launch("split_row_jobs_kernel"));
     }
-    const GatedOut out{raw ? wu : at(uh), at(ul), g, u, bu};
+    const GatedOut out{raw ? wu : at(uh), at(ul), g, u, bu, false};
     const Epilogue ep{bg, leaky_alpha, act, 0};
     KAI_TRY(run_tc(st, pl, h, at(xh), at(xl), raw ? wg : at(gh), at(gl), M, F, K, kp, F, ep, at(part), st->status_dev, s, mixed, &out));
     if (st->status_host[0] != 0)

@@ -267,9 +267,10 @@ struct Distill {
         }
     }
     __device__ __forceinline__ Result settle(const Parked* q, int slot, const Temp& tv) const {
-        double s = 0.0;
-#pragma unroll 4
-        for (int i = 0; i < 32; ++i) s += q->part[slot][i];
+        double s4[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s4[i & 3] += q->part[slot][i];
+        double s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         s = kLn2 * s + log_sum(q->total[slot]) - log_sum(q->weights[slot]);
         return Result{static_cast<float>(static_cast<double>(tv.t) * tv.t * s), 1.0f, 0.0f};
     }

@@ -14,21 +14,27 @@ from . import capi
 
 
 def _ptr(x):
-    if x is None:
-        return None
-    if isinstance(x, int):
-        return C.c_void_p(x)
+    if x is None or type(x) is int:        # ctypes turns integers into pointers
+        return x
     if hasattr(x, "data_ptr"):
         if not x.is_contiguous():
             raise ValueError("tensor arguments must be contiguous (the reference has no strides)")
-        return C.c_void_p(x.data_ptr())
+        return x.data_ptr()
+    if isinstance(x, int):
+        return int(x)
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 
+_type_names = {}     # torch.dtype -> its text, which torch puts together anew on every call
+
+
 def _typed(x, name):
-    """_ptr of an argument that is not fp32: a tensor of another type would be misread, not converted."""
-    if hasattr(x, "dtype") and str(x.dtype) != "torch." + name:
-        raise TypeError(f"a tensor of {name} is needed here, got {x.dtype}")
+    """_ptr of an argument that is not fp32 (`name`: the type's text): another type would be misread, not converted."""
+    if x is None or type(x) is int:
+        return x
+    kind = getattr(x, "dtype", None)
+    if kind is not None and _type_names.setdefault(kind, str(kind)) != name:
+        raise TypeError(f"a tensor of {name} is needed here, got {kind}")
     return _ptr(x)
 
 
@@ -266,7 +272,7 @@ def rotary(device, py, px, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot,
            ldx=None, stream=None):
     """Turns the pairs of every head by position * frequency; `layout` is "half" or "interleaved"."""
     nvec = nhead * npiece
-    capi.call("kai_rotary", device, _ptr(py), _ptr(px), _typed(pfreq, "float64"), _typed(ppos, "int64"), pos0, nbat, ntimes,
+    capi.call("kai_rotary", device, _ptr(py), _ptr(px), _typed(pfreq, "torch.float64"), _typed(ppos, "torch.int64"), pos0, nbat, ntimes,
               nhead, npiece, nrot, capi.ROTARY_LAYOUT[layout], _ptr(hScale), nvec if ldy is None else ldy,
               nvec if ldx is None else ldx, _ptr(stream))
 
@@ -274,7 +280,7 @@ def rotary(device, py, px, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot,
 def rotary_backward(device, pgx, pgy, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot, layout="half", hScale=None,
                     ldgx=None, ldgy=None, stream=None):
     nvec = nhead * npiece
-    capi.call("kai_rotary_backward", device, _ptr(pgx), _ptr(pgy), _typed(pfreq, "float64"), _typed(ppos, "int64"), pos0,
+    capi.call("kai_rotary_backward", device, _ptr(pgx), _ptr(pgy), _typed(pfreq, "torch.float64"), _typed(ppos, "torch.int64"), pos0,
               nbat, ntimes, nhead, npiece, nrot, capi.ROTARY_LAYOUT[layout], _ptr(hScale), nvec if ldgx is None else ldgx,
               nvec if ldgy is None else ldgy, _ptr(stream))
 
@@ -282,7 +288,7 @@ def rotary_backward(device, pgx, pgy, pfreq, ppos, pos0, nbat, ntimes, nhead, np
 def rotary_frequencies(device, pfreq, nrot, base=10000.0, scaling="plain", factor=1.0, slow=1.0, fast=32.0, times=1,
                        stream=None):
     """nrot / 2 doubles, radians per position; `scaling` is "plain", "linear", "base" or "by_parts"."""
-    capi.call("kai_rotary_frequencies", device, _typed(pfreq, "float64"), nrot, base, capi.ROTARY_SCALING[scaling], factor,
+    capi.call("kai_rotary_frequencies", device, _typed(pfreq, "torch.float64"), nrot, base, capi.ROTARY_SCALING[scaling], factor,
               slow, fast, times, _ptr(stream))
 
 
@@ -302,30 +308,30 @@ def gated_linear_backward(device, pgx, pgwg, pgwu, pgg, pgu, pgh, pg, pu, pwg, p
 
 def softmax_top_distill(device, py, ps, px, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
     """py[r] = temp^2 * KL(teacher's listed entries || softmax(px[r] / temp)); ps[nrow, 3] is for the backward call."""
-    capi.call("kai_softmax_top_distill", device, _ptr(py), _ptr(ps), _ptr(px), _typed(pidx, "int32"), _ptr(pt), nrow, ncol,
+    capi.call("kai_softmax_top_distill", device, _ptr(py), _ptr(ps), _ptr(px), _typed(pidx, "torch.int32"), _ptr(pt), nrow, ncol,
               ntop, _ptr(hTemp), _ptr(stream))
 
 
 def softmax_top_distill_backward_x(device, pgx, pgy, px, ps, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
     capi.call("kai_softmax_top_distill_backward_x", device, _ptr(pgx), _ptr(pgy), _ptr(px), _ptr(ps),
-              _typed(pidx, "int32"), _ptr(pt), nrow, ncol, ntop, _ptr(hTemp), _ptr(stream))
+              _typed(pidx, "torch.int32"), _ptr(pt), nrow, ncol, ntop, _ptr(hTemp), _ptr(stream))
 
 
 def softmax_top_distill_step(device, py, pgx, pgy, px, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
     """Loss and gradient with one read of the logits, for a pgy that is known beforehand (None: 1 for every row)."""
-    capi.call("kai_softmax_top_distill_step", device, _ptr(py), _ptr(pgx), _ptr(pgy), _ptr(px), _typed(pidx, "int32"),
+    capi.call("kai_softmax_top_distill_step", device, _ptr(py), _ptr(pgx), _ptr(pgy), _ptr(px), _typed(pidx, "torch.int32"),
               _ptr(pt), nrow, ncol, ntop, _ptr(hTemp), _ptr(stream))
 
 
 def softmax_policy_loss(device, py, plogp, ps, px, pz, pold, pref, padv, nrow, ncol, hClipLow=None, hClipHigh=None,
                         hKlCoef=None, hTemp=None, stream=None):
     """Clipped policy loss of the tokens pz, with a KL term against pref; plogp receives their log-probabilities."""
-    capi.call("kai_softmax_policy_loss", device, _ptr(py), _ptr(plogp), _ptr(ps), _ptr(px), _typed(pz, "int32"), _ptr(pold),
+    capi.call("kai_softmax_policy_loss", device, _ptr(py), _ptr(plogp), _ptr(ps), _ptr(px), _typed(pz, "torch.int32"), _ptr(pold),
               _ptr(pref), _ptr(padv), nrow, ncol, _ptr(hClipLow), _ptr(hClipHigh), _ptr(hKlCoef), _ptr(hTemp), _ptr(stream))
 
 
 def softmax_policy_loss_backward_x(device, pgx, pgy, px, ps, pz, nrow, ncol, hTemp=None, stream=None):
-    capi.call("kai_softmax_policy_loss_backward_x", device, _ptr(pgx), _ptr(pgy), _ptr(px), _ptr(ps), _typed(pz, "int32"),
+    capi.call("kai_softmax_policy_loss_backward_x", device, _ptr(pgx), _ptr(pgy), _ptr(px), _ptr(ps), _typed(pz, "torch.int32"),
               nrow, ncol, _ptr(hTemp), _ptr(stream))
 
 
@@ -333,7 +339,7 @@ def softmax_policy_loss_step(device, py, plogp, pgx, pgy, px, pz, pold, pref, pa
                              hClipHigh=None, hKlCoef=None, hTemp=None, stream=None):
     """Loss and gradient with one read of the logits, for a pgy that is known beforehand (None: 1 for every row)."""
     capi.call("kai_softmax_policy_loss_step", device, _ptr(py), _ptr(plogp), _ptr(pgx), _ptr(pgy), _ptr(px),
-              _typed(pz, "int32"), _ptr(pold), _ptr(pref), _ptr(padv), nrow, ncol, _ptr(hClipLow), _ptr(hClipHigh),
+              _typed(pz, "torch.int32"), _ptr(pold), _ptr(pref), _ptr(padv), nrow, ncol, _ptr(hClipLow), _ptr(hClipHigh),
               _ptr(hKlCoef), _ptr(hTemp), _ptr(stream))
 
 
