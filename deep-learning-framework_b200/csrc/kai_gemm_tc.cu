@@ -1937,6 +1937,17 @@ struct Carve {
     int64_t take(int64_t bytes) { const int64_t at = used; used += round_up(bytes, 256); return at; }
 };
 
+// The gated layer's three-TF32 products promote after 64 values of the reduction instead of up to 128: its gradients pass the
+// error of the projections on, and the truncation's share of it is what can be had for little (6749 rows, weight
+// gradient of 110 x 2968: 1.1e-6 of the result before, 7e-7 so; a chunk's MMAs still take longer than its promotion).
+// For the same reason they take the mixed scheme only from 4096 values on: at 2048 its cross terms leave 7.5e-7, three TF32
+// products 4e-7.
+constexpr int64_t kGatedCrossMinK = 4096;
+static void promote_early(TcPlan* pl, bool mixed) {
+    const int most = 64 / pl->bk;
+    if (!mixed && options().tc_kc.load() <= 0 && pl->kc_blocks > most) pl->kc_blocks = most;
+}
+
 int gated_forward_tc(DeviceState* st, int device, float* h, float* g, float* u, const float* wg, const float* wu, const float* x,
                      const float* bg, const float* bu, int64_t F, int64_t M, int64_t K, int act, const float* leaky_alpha,
                      cudaStream_t s) {
@@ -1947,6 +1958,7 @@ int gated_forward_tc(DeviceState* st, int device, float* h, float* g, float* u, 
     if ((K & 3) == 0 && M <= options().gated_raw_rows.load() &&
         ((reinterpret_cast<uintptr_t>(wg) | reinterpret_cast<uintptr_t>(wu) | reinterpret_cast<uintptr_t>(x)) & 15) == 0) {
         KAI_TRY(plan_tc(st, M, (F + UNITS - 1) / UNITS * 2 * UNITS, K, &pl, 0, true, true));
+        promote_early(&pl, false);
         const int64_t bytes = pl.slots * BM * pl.bn * 4;
         if (bytes > 0) KAI_TRY(ensure_workspace(st, device, bytes));
         const GatedOut out{wu, nullptr, g, u, bu, true};
@@ -1958,7 +1970,8 @@ int gated_forward_tc(DeviceState* st, int device, float* h, float* g, float* u, 
         return KAI_OK;
     }
     KAI_TRY(plan_tc(st, M, (F + UNITS - 1) / UNITS * 2 * UNITS, K, &pl, 0, true));
-    const bool mixed = options().tc_cross_bf16.load() != 0 && K >= kCrossMinK && (K & 7) == 0;
+    const bool mixed = options().tc_cross_bf16.load() != 0 && K >= kGatedCrossMinK && (K & 7) == 0;
+    promote_early(&pl, mixed);
     // A weight whose rows TMA can read serves as its own hi plane where its split is a visible share of the call (as in
     // gemm_tc; not in the mixed scheme, whose cross terms want rounded hi parts on the right side).
     const bool raw = options().tc_raw_hi.load() != 2 && !mixed && (K & 3) == 0 && M <= 2048 &&
@@ -2001,18 +2014,20 @@ int gated_backward_tc(DeviceState* st, int device, float* gx, float* gwg, float*
     p.mp = round_up(M, 4);
     p.act = act;
     const bool cross = options().tc_cross_bf16.load() != 0;
-    p.mixed_x = cross && 2 * p.fp >= kCrossMinK;
-    p.mixed_w = cross && M >= kCrossMinK && (M & 7) == 0;
+    p.mixed_x = cross && 2 * p.fp >= kGatedCrossMinK;
+    p.mixed_w = cross && M >= kGatedCrossMinK && (M & 7) == 0;
     TcPlan px{}, pw{};
     Carve ws;
     int64_t dh = 0, dl = 0, wh = 0, wl = 0, th = 0, tl = 0, xh = 0, xl = 0;
     if (gx) {
         KAI_TRY(plan_tc(st, M, K, 2 * p.fp, &px));
+        promote_early(&px, p.mixed_x != 0);
         dh = ws.take(M * 2 * p.fp * 4); dl = ws.take(M * 2 * p.fp * 4);
         wh = ws.take(K * 2 * p.fp * 4); wl = ws.take(K * 2 * p.fp * 4);
     }
     if (gwg) {
         KAI_TRY(plan_tc(st, 2 * F, K, M, &pw));
+        promote_early(&pw, p.mixed_w != 0);
         th = ws.take(2 * F * p.mp * 4); tl = ws.take(2 * F * p.mp * 4);
         xh = ws.take(K * p.mp * 4); xl = ws.take(K * p.mp * 4);
     }

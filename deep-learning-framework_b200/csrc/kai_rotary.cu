@@ -128,10 +128,11 @@ int launch(const RotaryParams& p0, bool half, bool in_place, int sm_count, cudaS
     const int rest = in_place ? 0 : p.npiece - p.nrot;
     p.units = p.rot_units + (rest + 2 * V - 1) / (2 * V);
     if (p.units == 0) return KAI_OK;
-    // Heads are shared out among threads until there are two full rounds of threads; then every thread walks over more
-    // heads per angle.
-    const int64_t target = static_cast<int64_t>(sm_count) * 2048 * 2;
-    int64_t groups = (target + p.rows * p.units - 1) / (p.rows * p.units);
+    // Four heads per thread and angle, fewer where that leaves the SMs' thread slots empty.  3 x 32771 tokens, 12 heads: 123 us with
+    // 3 or 4 heads per thread, 132 with 12, 166 with one; 32 x 512 tokens, 8 heads: 16.6 us with 2 to 8, 20 with one.
+    const int64_t slots = static_cast<int64_t>(sm_count) * 2048;
+    int64_t groups = (slots + p.rows * p.units - 1) / (p.rows * p.units);
+    if (groups < (p.nhead + 3) / 4) groups = (p.nhead + 3) / 4;
     if (groups > p.nhead) groups = p.nhead;
     p.head_groups = static_cast<int>(groups);
     const int64_t blocks = (p.rows * p.units * groups + 255) / 256;

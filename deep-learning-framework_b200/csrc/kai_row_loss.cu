@@ -160,11 +160,12 @@ struct Distill {
     int ntop, ntop4;       // ntop4: rounded up to a multiple of 4, unused entries behind ntop
 
     struct Row : RowHead {};
-    __host__ __device__ size_t bytes() const { return sizeof(RowHead) + 16 * static_cast<size_t>(ntop4); }
+    __host__ __device__ size_t bytes() const { return sizeof(RowHead) + 20 * static_cast<size_t>(ntop4); }
     static __device__ __forceinline__ int* ids(Row* r) { return reinterpret_cast<int*>(r + 1); }
     __device__ __forceinline__ float* probs(Row* r) const { return reinterpret_cast<float*>(ids(r) + ntop4); }
     __device__ __forceinline__ float* logits(Row* r) const { return probs(r) + ntop4; }
     __device__ __forceinline__ float* teacher(Row* r) const { return logits(r) + ntop4; }
+    __device__ __forceinline__ float* merged(Row* r) const { return teacher(r) + ntop4; }
     __device__ __forceinline__ int labels() const { return ntop; }
 
     // The label warp works ahead so that no load of its own is waited for: ids and teacher logits are fetched two rows ahead
@@ -198,7 +199,7 @@ struct Distill {
     // One warp: labels and logits into shared memory, the teacher's entries as probabilities (0 for unused entries), and
     // the row's state.
     __device__ __forceinline__ void arrive(Row* r, const Flight& f, const Ahead& a, const float* x, const RowShape& shape,
-                                           int part, bool all, int64_t row, int64_t ncol, const Temp& tv) const {
+                                           int part, bool all, int64_t row, int64_t ncol, const Temp& tv, bool gradient) const {
         const int lane = threadIdx.x & 31;
         int* id = ids(r);
         float* p = probs(r);
@@ -238,6 +239,16 @@ struct Distill {
         sum = warp_sum(sum);
         const float inv = some ? 1.0f / sum : 0.0f;
         for (int j = lane; j < ntop4; j += 32) p[j] *= inv;
+        if (gradient && ntop <= kMergeAhead) {
+            // repeated ids: the first place of an id takes the sum, the others are marked
+            __syncwarp();
+            for (int j = lane; j < ntop; j += 32) {
+                int first = j;
+                float sum_j = 0.0f;
+                if (id[j] >= 0) search(r, id[j], 0, 1, first, sum_j);
+                merged(r)[j] = (id[j] >= 0 && first == j) ? sum_j : -1.0f;
+            }
+        }
         if (lane == 0) {
             r->teacher = k;
             r->weights = sum;
@@ -276,39 +287,51 @@ struct Distill {
     }
     __device__ __forceinline__ float finish_slope(Row*, float, float, const Temp&) const { return 1.0f; }
     __device__ __forceinline__ float coef(Row* r, float, const Temp& tv) const { return r->gy * tv.t; }
+    // Up to this many labels the label warp joins repeated ids while it waits for the others anyway (as part of the gradient's pass
+    // it cost 3500 clocks per row at 64 labels); beyond, its time would grow with the square, and all threads share it.
+    static constexpr int kMergeAhead = 128;
+    // Places of id z: the first of them, and the sum of their probabilities.  Thread `sub` of `g` looks at every g-th group of four.
+    __device__ __forceinline__ void search(Row* r, int z, int sub, int g, int& first, float& sum) const {
+        const int4* id4 = reinterpret_cast<const int4*>(ids(r));
+        const float4* p4 = reinterpret_cast<const float4*>(probs(r));
+#pragma unroll 4
+        for (int i = sub; i < ntop4 / 4; i += g) {
+            const int4 v = id4[i];
+            if (v.x == z || v.y == z || v.z == z || v.w == z) {
+                const float4 q = p4[i];
+                if (v.x == z) { sum += q.x; first = min(first, 4 * i); }
+                if (v.y == z) { sum += q.y; first = min(first, 4 * i + 1); }
+                if (v.z == z) { sum += q.z; first = min(first, 4 * i + 2); }
+                if (v.w == z) { sum += q.w; first = min(first, 4 * i + 3); }
+            }
+        }
+    }
     // Threads that share the search for one label's repetitions: a power of two up to 32, `threads` being a multiple of 32.
     __device__ __forceinline__ int sharers(int threads) const {
         int g = 1;
-        while (g < 32 && 2 * g * ntop <= threads) g *= 2;
+        while (ntop > kMergeAhead && g < 32 && 2 * g * ntop <= threads) g *= 2;
         return g;
     }
-    // Label j's column and weight; an id that occurs again belongs to its first place.  Called by whole warps: thread `sub` of
-    // `g` neighbours looks through every g-th group of four entries, in an order that g alone determines.
+    // Label j's column and weight; an id that occurs again belongs to its first place.  Called by whole warps.
     __device__ __forceinline__ bool label(Row* r, int j, int sub, int g, int& c, float& w, float& x) const {
         const int z = j < ntop ? ids(r)[j] : -1;
+        c = z;
+        if (ntop <= kMergeAhead) {
+            if (z < 0) return false;
+            w = merged(r)[j];
+            x = logits(r)[j];
+            return w >= 0.0f || isnan(w);
+        }
         int first = j;
         float sum = 0.0f;
         if (z >= 0) {
-            const int4* id4 = reinterpret_cast<const int4*>(ids(r));
-            const float4* p4 = reinterpret_cast<const float4*>(probs(r));
-#pragma unroll 4
-            for (int i = sub; i < ntop4 / 4; i += g) {
-                const int4 v = id4[i];
-                if (v.x == z || v.y == z || v.z == z || v.w == z) {
-                    const float4 q = p4[i];
-                    if (v.x == z) { sum += q.x; first = min(first, 4 * i); }
-                    if (v.y == z) { sum += q.y; first = min(first, 4 * i + 1); }
-                    if (v.z == z) { sum += q.z; first = min(first, 4 * i + 2); }
-                    if (v.w == z) { sum += q.w; first = min(first, 4 * i + 3); }
-                }
-            }
+            search(r, z, sub, g, first, sum);
             x = logits(r)[j];
         }
         for (int o = 1; o < g; o *= 2) {
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
             first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
         }
-        c = z;
         w = sum;
         return z >= 0 && first == j && sub == 0;
     }
@@ -350,7 +373,7 @@ struct Policy {
         f.adv = (adv != nullptr) ? adv[row] : 0.0f;
     }
     __device__ __forceinline__ void arrive(Row* r, const Flight& f, const Ahead& a, const float*, const RowShape&, int, bool,
-                                           int64_t, int64_t ncol, const Temp&) const {
+                                           int64_t, int64_t ncol, const Temp&, bool) const {
         if ((threadIdx.x & 31) == 0) {
             r->id = a.id;
             r->state = (a.id >= 0 && a.id < ncol) ? kLive : (a.id == -1 ? kPadding : kBad);
@@ -531,7 +554,7 @@ row_stream_kernel(const RowParams p, const L loss) {
         Row* r = reinterpret_cast<Row*>(rows + buf * row_bytes);
         if (lane == 0) r->gy = gy_next;
         if (MODE == kGrad && lane < 3) r->stat[lane] = ps_next;
-        loss.arrive(r, flight, ids, x, shape, part, MODE != kGrad, row, p.ncol, tv);
+        loss.arrive(r, flight, ids, x, shape, part, MODE != kGrad, row, p.ncol, tv, MODE != kLoss);
     };
 
     if (first < p.nrow) {
@@ -693,7 +716,7 @@ row_loss_wide_kernel(const RowParams p, const L loss) {
             typename L::Flight flight;
             loss.ahead(ids, row);
             loss.depart(flight, ids, x, shape, part, true, row, p.ncol);
-            loss.arrive(r, flight, ids, x, shape, part, true, row, p.ncol, tv);
+            loss.arrive(r, flight, ids, x, shape, part, true, row, p.ncol, tv, false);
         }
     } else {
         const float4* xq = reinterpret_cast<const float4*>(x + shape.head);
@@ -738,7 +761,8 @@ row_loss_wide_kernel(const RowParams p, const L loss) {
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------
-constexpr int64_t kPart = 8192;       // columns of a part: 32 KB, five or six parts to an SM
+constexpr int64_t kPart = 12800;      // columns of a part at most, where a row has several: 50 KB, four parts to an SM
+constexpr int64_t kPartOne = 16384;   // columns from which on a part is a matter for 256 threads
 constexpr size_t kSmemMost = 220 * 1024;
 
 // Clusters (or, for `parts` = 1, CTAs) of a kernel that are resident on the device at once: the size of a persistent grid.
@@ -840,12 +864,12 @@ int row_parts(int64_t nrow, int64_t ncol, int64_t most, int sm_count) {
     return static_cast<int>(parts);
 }
 
-// Threads of a CTA: 64 for many short rows (a part of 2048 columns at most), 256 for parts beyond kPart and where there are too few
-// parts to give every SM four, 128 otherwise.
+// Threads of a CTA: 64 for many short rows (a part of 2048 columns at most), 256 for parts beyond kPartOne and where there are too
+// few parts to give every SM four, 128 otherwise.
 template <class L, int MODE>
 int launch_threads(DeviceState* st, const RowParams& p, const L& loss, cudaStream_t s) {
     const int64_t each = (p.ncol + p.parts - 1) / p.parts, ctas = p.nrow * p.parts;
-    if (each > kPart || ctas < 4 * static_cast<int64_t>(st->sm_count)) return launch_stream<L, 256, MODE>(st, p, loss, s);
+    if (each > kPartOne || ctas < 4 * static_cast<int64_t>(st->sm_count)) return launch_stream<L, 256, MODE>(st, p, loss, s);
     if (each <= 2048) return launch_stream<L, 64, MODE>(st, p, loss, s);
     return launch_stream<L, 128, MODE>(st, p, loss, s);
 }
