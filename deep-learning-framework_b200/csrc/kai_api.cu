@@ -1486,7 +1486,7 @@ int kai_gated_linear_forward(int device, float* ph, float* pg, float* pu, const 
     const double flops = 4.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
     if (gated_skinny_takes(ndat, xvec, px, pwg, pwu))
         return gated_skinny(st, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
-    if (xvec > 0 && ndat > 16 && flops >= static_cast<double>(options().gated_tc_flops.load()))
+    if (ndat > 16 && yvec >= 32 && xvec >= 32 && flops >= static_cast<double>(options().gated_tc_flops.load()))
         return gated_forward_tc(st, device, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
     return gated_forward_mma(st, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
 }
@@ -1515,7 +1515,7 @@ int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float* pgwu, 
     if (clash) return fail(KAI_E_INVALID_ARG, "gated_linear_backward: two buffers overlap");
     KAI_ENTER(device);
     const double flops = 4.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
-    if (ndat > 16 && flops > 0.0 && flops >= static_cast<double>(options().gated_tc_flops.load()) && (pgx || pgwg))
+    if (ndat > 16 && yvec >= 32 && xvec >= 32 && flops >= static_cast<double>(options().gated_tc_flops.load()) && (pgx || pgwg))
         return gated_backward_tc(st, device, pgx, pgwg, pgwu, pgg, pgu, pgh, pg, pu, pwg, pwu, px, yvec, ndat, xvec, act,
                                  leaky_alpha, acc_x, acc_w, s);
     if (ndat * yvec > 0)

@@ -90,9 +90,9 @@ __device__ __forceinline__ V warp_sum(V v) {
     return v;
 }
 
-// log of a positive sum, to about 1e-8 absolute
+// log of a positive sum, to about 1e-8 absolute; NaN for a sum of nothing
 __device__ __forceinline__ double log_sum(float s) {
-    if (!(s > 0.0f) || isinf(s)) return static_cast<double>(logf(s));
+    if (!(s > 0.0f) || isinf(s)) return static_cast<double>(nanf(""));     // no distribution
     int e;
     float f = frexpf(s, &e);
     if (f < 0.70710678f) { f *= 2.0f; --e; }
@@ -306,10 +306,10 @@ struct Distill {
             }
         }
     }
-    // Threads that share the search for one label's repetitions: a power of two up to 32, `threads` being a multiple of 32.
+    // Threads that share the search for one label's repetitions, as a power of two (32 at most), `threads` being a multiple of 32.
     __device__ __forceinline__ int sharers(int threads) const {
-        int g = 1;
-        while (ntop > kMergeAhead && g < 32 && 2 * g * ntop <= threads) g *= 2;
+        int g = 0;
+        while (ntop > kMergeAhead && g < 5 && (ntop << (g + 1)) <= threads) ++g;
         return g;
     }
     // Label j's column and weight; an id that occurs again belongs to its first place.  Called by whole warps.
@@ -412,7 +412,7 @@ struct Policy {
     __device__ __forceinline__ float coef(Row* r, float slope, const Temp& tv) const {
         return -(r->gy * slope) / tv.t;
     }
-    __device__ __forceinline__ int sharers(int) const { return 1; }
+    __device__ __forceinline__ int sharers(int) const { return 0; }
     __device__ __forceinline__ bool label(Row* r, int j, int, int, int& c, float& w, float& x) const {
         c = r->id;
         w = 1.0f;
@@ -650,11 +650,11 @@ row_stream_kernel(const RowParams p, const L loss) {
                 asm volatile("bar.sync 1, %0;" ::"n"(T) : "memory");
                 // the labels' columns, over what has just been written there
                 const int g = loss.sharers(T);
-                for (int j0 = 0; j0 < loss.labels(); j0 += T / g) {
-                    const int j = j0 + tid / g;
+                for (int j0 = 0; j0 < loss.labels(); j0 += T >> g) {
+                    const int j = j0 + (tid >> g);
                     int c;
                     float w, xv;
-                    if (loss.label(r, j, tid % g, g, c, w, xv) && shape.owned(c, part)) {
+                    if (loss.label(r, j, tid & ((1 << g) - 1), 1 << g, c, w, xv) && shape.owned(c, part)) {
                         const float v = weight(xv, kf, tv.c) * f - coef * w;
                         const int q = (c - shape.head) >> 2;
                         if (c < shape.head) loose_sh[c] = v;
@@ -770,13 +770,16 @@ constexpr size_t kSmemMost = 220 * 1024;
 int resident_clusters(const void* kernel, int threads, int parts, size_t smem, int sm_count, int* out) {
     struct Known { const void* kernel; int device, parts; size_t smem; int clusters; };
     static std::mutex mu;
-    static std::vector<Known> known;
+    static Known known[64];          // the first of them; what does not fit any more is asked again
+    static int count = 0;
     int device = 0;
     KAI_CUDA(cudaGetDevice(&device));
     {
         std::lock_guard<std::mutex> lock(mu);
-        for (const Known& k : known)
+        for (int i = 0; i < count; ++i) {
+            const Known& k = known[i];
             if (k.kernel == kernel && k.device == device && k.parts == parts && k.smem == smem) { *out = k.clusters; return KAI_OK; }
+        }
     }
     KAI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMost)));
     int clusters = 0;
@@ -801,7 +804,7 @@ int resident_clusters(const void* kernel, int threads, int parts, size_t smem, i
     if (clusters < 1) return fail(KAI_E_TOO_LARGE, "row losses: %zu bytes of shared memory do not fit", smem);
     *out = clusters;
     std::lock_guard<std::mutex> lock(mu);
-    known.push_back(Known{kernel, device, parts, smem, clusters});
+    if (count < 64) known[count++] = Known{kernel, device, parts, smem, clusters};
     return KAI_OK;
 }
 

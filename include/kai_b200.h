@@ -99,6 +99,9 @@ KAI_API int kai_selftest_bounded_wait(int device, int64_t limit_ns, void* stream
  * "tc_pair" (1, the default: products whose 256 x 256 tiles fill at least half a round of the SM pairs run on
  * pairs of CTAs with cta_group::2 MMAs -- 8192^3: 3.65 ms against 4.35 ms with one CTA per 128 x 256 tile; 0 = one
  * CTA per tile always), "tc_pair_bk" (K block of the pair kernel, 32 or 16).
+ * "gated_tc_flops" (flops 4 ndat xvec yvec of a gated layer from which on its products run on the tensor-core GEMM instead of the
+ * one-launch warp-level kernels), "gated_raw_rows" (most rows for which that GEMM's forward form reads the operands as they
+ * are instead of writing planes first).
  * Returns KAI_E_INVALID_ARG for an unknown name or value. */
 KAI_API int kai_set_option(const char* name, int64_t value);
 KAI_API int64_t kai_get_option(const char* name);
@@ -464,7 +467,9 @@ KAI_API int kai_rotary_frequencies(int device, double* pfreq, int64_t nrot, doub
  *   pgg = pgh * u * act'(g),   pgu = pgh * act(g)        (written; a bias gradient is kai_add_bias_backward_b of them)
  *   pgx (+)= pgg . pwg + pgu . pwu,   pgwg (+)= pgg^T . px,   pgwu (+)= pgu^T . px
  * acc_x / acc_w: += instead of =.  pgx may be NULL (input without gradient), and pgwg together with pgwu (fixed
- * weights).  pgg and pgu may alias pg and pu, or pgh one of the two; other overlaps are not allowed. */
+ * weights).  pgg and pgu may alias pg and pu, or pgh one of the two; other overlaps are not allowed.  The products have the
+ * accuracy of kai_matmul's: operands are split into TF32 parts, so an infinity may come out as NaN (in its own row, or
+ * in its own weight's column). */
 KAI_API int kai_gated_linear_forward(int device, float* ph, float* pg, float* pu, const float* pwg, const float* pwu,
                                      const float* px, const float* pbg, const float* pbu, int64_t yvec, int64_t ndat,
                                      int64_t xvec, int act, const float* leaky_alpha, void* stream);
@@ -474,13 +479,15 @@ KAI_API int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float
                                       int act, const float* leaky_alpha, int acc_x, int acc_w, void* stream);
 
 /* Losses on rows of logits px[nrow,ncol], with q = softmax(px[r,:] / temp).  temp is a HYPER (> 0), except that NULL
- * reads as 1.  Each comes as a forward call that saves three numbers per row in ps[nrow,3] (row maximum, sum of
- * exponentials, d loss / d log-probability), a backward call that reads them, and a _step call that does both with one
- * read of px, for callers that know the loss's gradient pgy[nrow] beforehand (NULL reads as 1 for every row).  pgx may
+ * reads as 1.  Each comes as a forward call that saves three numbers per row in ps[nrow,3] (the exponent that the row's
+ * exponentials are taken against, their sum, d loss / d log-probability), a backward call that reads them, and a _step call
+ * that does both with one read of px, for callers that know the loss's gradient pgy[nrow] beforehand (NULL reads as 1
+ * for every row).  pgx may
  * be px itself in the backward and _step calls; any other overlap is not allowed.  Rows without a label
  * (pz[r] = -1, or no used entry that has a weight) are padding: loss and gradient 0, whatever the logits hold.  Labels are checked on
  * the device: any other label outside [0, ncol) makes the row's loss and gradient NaN and is reported by
- * kai_device_status (KAI_E_OUT_OF_RANGE).
+ * kai_device_status (KAI_E_OUT_OF_RANGE).  A logit of -inf, or one so low that logit / temp * log2(e) leaves the range of
+ * fp32, has probability 0; a labelled row of nothing else has no distribution and comes out NaN.
  *
  * Distillation from a teacher's top logits: pidx[nrow,ntop] names the columns, pt[nrow,ntop] holds the teacher's
  * logits (or log-probabilities) there; unused entries have id -1, and an entry of -inf has no weight.  An id that

@@ -82,7 +82,8 @@ def _forward(torch, vm, d, m, k, f, act, save=True, alpha=None, stream=None):
 SHAPES = [(1, 1, 1), (1, 64, 96), (1, 4096, 128), (1, 257, 65), (2, 512, 130), (3, 1028, 77), (4, 256, 8), (7, 100, 33),
           (8, 1024, 64), (15, 2052, 129), (16, 512, 512), (17, 512, 96), (33, 130, 70), (48, 1024, 200), (64, 4096, 64),
           (100, 96, 300), (129, 257, 255), (391, 512, 1365), (256, 512, 1024), (2048, 64, 64), (300, 1000, 700),
-          (1024, 1024, 1024), (1153, 2048, 640), (5, 3, 4096), (640, 2056, 515)]
+          (1024, 1024, 1024), (1153, 2048, 640), (5, 3, 4096), (640, 2056, 515), (300, 1000, 1100), (300, 1001, 1100),
+          (1290, 520, 1030), (1280, 4104, 1024), (4104, 256, 520)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -101,6 +102,33 @@ def test_forward_and_gradients(torch_cuda, vm, shape):
     torch.cuda.synchronize()
     _check(vals, tols, dict(h=h, g=g, u=u, gg=gg, gu=gu, gx=gx, gwg=gwg, gwu=gwu))
     assert torch.equal(h, h2)                    # saving the factors does not change the result
+
+
+@pytest.mark.parametrize("path", ["warp", "planes", "raw"])
+@pytest.mark.parametrize("shape", [(17, 33, 35), (20, 64, 32), (33, 132, 70), (100, 96, 300), (129, 257, 255), (200, 300, 130), (700, 40, 48)])
+def test_every_kernel_at_odd_sizes(torch_cuda, pkg, vm, shape, path):
+    """The sizes at which the dispatch changes kernels, moved out of the way."""
+    torch = torch_cuda
+    m, k, f = shape
+    a = _inputs(m, k, f, True, m)
+    vals, tols = _truth(torch, a, "swish")
+    d = _dev(torch, a)
+    old = [pkg.load().kai_get_option(n) for n in (b"gated_tc_flops", b"gated_raw_rows")]
+    pkg.capi.call("kai_set_option", b"gated_tc_flops", (1 << 62) if path == "warp" else 0)
+    pkg.capi.call("kai_set_option", b"gated_raw_rows", (1 << 40) if path == "raw" else 0)
+    try:
+        h, g, u = _forward(torch, vm, d, m, k, f, "swish")
+        h2, _, _ = _forward(torch, vm, d, m, k, f, "swish", save=False)
+        gx, gwg, gwu = _new(torch, m, k), torch.ones((f, k), device="cuda"), torch.zeros((f, k), device="cuda")
+        gg, gu = _new(torch, m, f), _new(torch, m, f)
+        vm.gated_linear_backward(0, gx, gwg, gwu, gg, gu, d["gh"], g, u, d["wg"], d["wu"], d["x"], f, m, k, "swish", acc_w=True)
+        torch.cuda.synchronize()
+    finally:
+        pkg.capi.call("kai_set_option", b"gated_tc_flops", old[0])
+        pkg.capi.call("kai_set_option", b"gated_raw_rows", old[1])
+    tols["gwg"] += 2 * U * float((vals["gwg"].abs() + 1).norm())        # the addition's rounding, and the subtraction's
+    _check(vals, tols, dict(h=h, g=g, u=u, gg=gg, gu=gu, gx=gx, gwg=gwg - 1, gwu=gwu))
+    assert torch.equal(h, h2)
 
 
 @pytest.mark.parametrize("act", ACTS)

@@ -158,6 +158,19 @@ def test_distill_infinities(torch_cuda, vm, mode, ncol):
     assert np.isnan(y[4])
 
 
+@pytest.mark.parametrize("mode", ["step", "calls"])
+def test_rows_without_a_distribution_and_tables_without_entries(torch_cuda, vm, mode):
+    torch = torch_cuda
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((3, 50)).astype(np.float32)
+    x[0], x[1] = -np.inf, np.finfo(np.float32).min
+    idx, t = _table(rng, 3, 50, 4)
+    y, gx = _run_distill(torch, vm, mode, x, idx, t, 1.0, np.ones(3, np.float32))
+    assert np.isnan(y[:2]).all() and np.isnan(gx[:2]).all() and np.isfinite(y[2]) and np.isfinite(gx[2]).all()
+    y, gx = _run_distill(torch, vm, mode, x, np.zeros((3, 0), np.int32), np.zeros((3, 0), np.float32), 1.0, np.ones(3, np.float32))
+    assert np.all(y == 0) and np.all(gx == 0)
+
+
 def test_distill_gradient_against_differences(torch_cuda, vm):
     """Central differences of the kernel's own loss.  The loss is about 20, off by 1e-5 at most; h = 0.05 leaves h^2 / 6 times a third
     derivative below temp^-1 = 1/2 in size: 1e-5 / 0.05 + 0.0025 / 12 < 6e-4."""
