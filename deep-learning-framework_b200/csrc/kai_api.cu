@@ -57,7 +57,7 @@ int gated_forward_tc(DeviceState*, int, float*, float*, float*, const float*, co
 int gated_backward_tc(DeviceState*, int, float*, float*, float*, float*, float*, const float*, const float*, const float*,
                       const float*, const float*, const float*, int64_t, int64_t, int64_t, int, const float*, int, int,
                       cudaStream_t);
-bool gated_skinny_takes(int64_t, int64_t, const float*, const float*, const float*);
+bool gated_skinny_takes(int64_t, int64_t, int64_t, const float*, const float*, const float*);
 int gated_skinny(DeviceState*, float*, float*, float*, const float*, const float*, const float*, const float*, const float*,
                  int64_t, int64_t, int64_t, int, const float*, cudaStream_t);
 int gated_forward_mma(DeviceState*, float*, float*, float*, const float*, const float*, const float*, const float*, const float*,
@@ -1484,7 +1484,7 @@ int kai_gated_linear_forward(int device, float* ph, float* pg, float* pu, const 
     KAI_ENTER(device);
     if (ndat == 0 || yvec == 0) return KAI_OK;
     const double flops = 4.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
-    if (gated_skinny_takes(ndat, xvec, px, pwg, pwu))
+    if (gated_skinny_takes(yvec, ndat, xvec, px, pwg, pwu))
         return gated_skinny(st, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);
     if (ndat > 16 && yvec >= 32 && xvec >= 32 && flops >= static_cast<double>(options().gated_tc_flops.load()))
         return gated_forward_tc(st, device, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act, leaky_alpha, s);

@@ -327,6 +327,116 @@ skinny_fma_kernel(const float* __restrict__ x, const float* __restrict__ w, floa
     }
 }
 
+// The gated layer for 17 to 48 rows: the stream of skinny_mma_kernel with more column tiles per fragment of the weights; X comes from
+// L1 / L2 piece by piece, since the pieces of a whole step would not leave registers for the sums.  Every block reads all of X for
+// its 16 rows of weights, which bounds the kernel (4096 x 4096: 15 us per 8 rows of X, against 6 of tensor
+// instructions): up to 32 rows it is still the fastest form measured (20 rows: 48 us, tcgen05 kernel 62; 24 rows of 1024 x
+// 1024: 7.4, one-launch warp kernel 12.6), up to 48 where the weights are few (1024 x 1024: 10.6 against 12.6; 4096 x 4096:
+// 90 against 68).
+template <int NT>
+__global__ void __launch_bounds__(SKM_WARPS * 32, 2)
+gated_rows_kernel(const float* __restrict__ x, const float* __restrict__ wg, float* __restrict__ h, int M, int64_t N, int64_t K,
+                  const float* __restrict__ bias, const float* __restrict__ leaky_alpha, int act, const SkinnyGate gate) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 8;
+    const int64_t row = (n0 + g < N) ? (n0 + g) : (N - 1);       // rows past N are clamped (their results are never stored)
+    const float* w0 = wg + row * K + 4 * t;
+    const float* w1 = gate.wu + row * K + 4 * t;
+    const float* xp = x + static_cast<int64_t>(g) * K + 4 * t;   // column tile i: row g + 8 i
+    constexpr int64_t kStride = static_cast<int64_t>(SKM_WARPS) * SKM_STEP;
+
+    float acc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+
+    extern __shared__ float4 skm_ring[];          // [warp][stage][piece 0..7][lane]
+    float4* ring = skm_ring + static_cast<size_t>(warp) * SKM_STAGES * 8 * 32 + lane;
+    auto issue = [&](int64_t k0, int stage) {
+        float4* dst = ring + stage * 8 * 32;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t k = k0 + 16 * j;
+            const bool in = (k + 4 * t) < K;      // K % 4 == 0: a piece is inside or outside as a whole
+            cp_async16(dst + (2 * j) * 32, in ? (w0 + k) : w0, in);
+            cp_async16(dst + (2 * j + 1) * 32, in ? (w1 + k) : w1, in);
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int sidx = 0; sidx < SKM_STAGES - 1; ++sidx) issue(static_cast<int64_t>(warp) * SKM_STEP + sidx * kStride, sidx);
+    int stage = 0;
+    for (int64_t k0 = static_cast<int64_t>(warp) * SKM_STEP; k0 < K; k0 += kStride) {
+        issue(k0 + (SKM_STAGES - 1) * kStride, (stage == 0) ? SKM_STAGES - 1 : stage - 1);
+        cp_async_wait<SKM_STAGES - 1>();
+        float c[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[i][e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t k = k0 + 16 * j;
+            const bool in = (k + 4 * t) < K;
+            float4 xv[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+                xv[i] = (in && g + 8 * i < M) ? __ldg(reinterpret_cast<const float4*>(xp + static_cast<int64_t>(8 * i) * K + k))
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 wa = ring[(stage * 8 + 2 * j) * 32], wb = ring[(stage * 8 + 2 * j + 1) * 32];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t ah[4], al[4];
+                split_frag(half ? wa.z : wa.x, ah[0], al[0]);
+                split_frag(half ? wb.z : wb.x, ah[1], al[1]);
+                split_frag(half ? wa.w : wa.y, ah[2], al[2]);
+                split_frag(half ? wb.w : wb.y, ah[3], al[3]);
+                uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    split_frag(half ? xv[i].z : xv[i].x, bh[i][0], bl[i][0]);
+                    split_frag(half ? xv[i].w : xv[i].y, bh[i][1], bl[i][1]);
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i) mma_tf32(c[i], al, bh[i]);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) mma_tf32(c[i], ah, bl[i]);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) mma_tf32(c[i], ah, bh[i]);
+            }
+        }
+        if (++stage == SKM_STAGES) stage = 0;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][e] += c[i][e];
+    }
+    cp_async_wait<0>();
+    __syncthreads();                              // the ring becomes the warps' fragments: [warp][16][8 NT + 1]
+    float* red = reinterpret_cast<float*>(skm_ring);
+    constexpr int PITCH = 8 * NT + 1;
+    static_assert(SKM_WARPS * 16 * PITCH * 4 <= SKM_RING_BYTES, "fragments fit in the ring");
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            red[(warp * 16 + g + 8 * (e >> 1)) * PITCH + 8 * i + 2 * t + (e & 1)] = acc[i][e];
+    __syncthreads();
+    const float alpha = (leaky_alpha != nullptr) ? __ldg(leaky_alpha) : 0.0f;
+#pragma unroll 1
+    for (int e = threadIdx.x; e < 8 * 8 * NT; e += SKM_WARPS * 32) {
+        const int r = e & 7, m = e >> 3;
+        const int64_t n = n0 + r;
+        if (n >= N || m >= M) continue;
+        float sg = 0.0f, su = 0.0f;
+#pragma unroll
+        for (int ww = 0; ww < SKM_WARPS; ++ww) { sg += red[(ww * 16 + r) * PITCH + m]; su += red[(ww * 16 + r + 8) * PITCH + m]; }
+        store_gate(gate, h, static_cast<int64_t>(m) * N + n, n, sg, su, bias, act, alpha);
+    }
+}
+
 }  // namespace
 
 int gemm_skinny_mma(float* c, const float* x, const float* w, int64_t M, int64_t N, int64_t K, int64_t ldc,
@@ -375,8 +485,8 @@ int gemm_skinny_mma(float* c, const float* x, const float* w, int64_t M, int64_t
 }
 
 // The gated layer for a handful of rows: both weights streamed once, h = act(g) * u in the same launch.
-bool gated_skinny_takes(int64_t M, int64_t K, const float* x, const float* wg, const float* wu) {
-    return M >= 1 && M <= 16 && K >= 64 && (K & 3) == 0 &&
+bool gated_skinny_takes(int64_t F, int64_t M, int64_t K, const float* x, const float* wg, const float* wu) {
+    return M >= 1 && M <= (F * K <= (int64_t(1) << 22) ? 48 : 32) && K >= 64 && (K & 3) == 0 &&
            ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(wg) | reinterpret_cast<uintptr_t>(wu)) & 15) == 0;
 }
 int gated_skinny(DeviceState* st, float* h, float* g, float* u, const float* wg, const float* wu, const float* x, const float* bg,
@@ -390,6 +500,9 @@ int gated_skinny(DeviceState* st, float* h, float* g, float* u, const float* wg,
         KAI_CUDA(cudaFuncSetAttribute(skinny_fma_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
         KAI_CUDA(cudaFuncSetAttribute(skinny_fma_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
         KAI_CUDA(cudaFuncSetAttribute(skinny_fma_kernel<4, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
+        KAI_CUDA(cudaFuncSetAttribute(gated_rows_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
+        KAI_CUDA(cudaFuncSetAttribute(gated_rows_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
+        KAI_CUDA(cudaFuncSetAttribute(gated_rows_kernel<6>, cudaFuncAttributeMaxDynamicSharedMemorySize, SKM_RING_BYTES));
         configured[dev] = true;
     }
     const SkinnyGate gate{wu, bu, g, u};
@@ -403,6 +516,13 @@ int gated_skinny(DeviceState* st, float* h, float* g, float* u, const float* wg,
         if (M == 1) skinny_fma_kernel<1, true><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
         else if (M == 2) skinny_fma_kernel<2, true><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
         else skinny_fma_kernel<4, true><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
+#undef KAI_SKG_ARGS
+    } else if (M > 16) {
+        const unsigned grid = static_cast<unsigned>((F + 7) / 8);
+#define KAI_SKG_ARGS x, wg, h, m, F, K, bg, leaky_alpha, act, gate
+        if (M <= 24) gated_rows_kernel<3><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
+        else if (M <= 32) gated_rows_kernel<4><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
+        else gated_rows_kernel<6><<<grid, SKM_WARPS * 32, SKM_RING_BYTES, s>>>(KAI_SKG_ARGS);
 #undef KAI_SKG_ARGS
     } else {
         const unsigned grid = static_cast<unsigned>((F + 7) / 8);

@@ -26,10 +26,12 @@
 // row_loss_wide_kernel takes the rows that the shared memory of a cluster cannot hold (more than 400000 columns), for kLoss;
 // kStep is then kLoss and kGrad.
 //
-// Precision.  exp((x - m) / T) is formed as 2^(x c - k) with c = log2(e) / T rounded once and k the integer above m c: one
-// fused multiply-add, rounded relative to the exponent itself, and sums against different k are joined by exact powers of
-// two.  Rounding c is a temperature off by 2^-24, the same for every term.  Exponentials and their sums are fp32 (a few
-// dozen values per thread, then joined in a fixed order); log q = ln 2 (x c - k) - log(sum) is formed in 64 bits per row, with
+// Precision.  exp((x - m) / T) is formed as 2^(x c - k) with c = log2(e) / T and k = m c, each rounded once: one fused multiply-add,
+// rounded relative to the exponent itself; what k lost stands in every term and in the logarithm below alike, and rounding
+// c is a temperature off by 2^-24, the same for every term.  The largest term is 2^0 to within rounding: with k the integer above
+// m c, which joins sums by exact powers of two, it is a power of a fraction, and the instruction's 2^-22 on a term that is nearly
+// the whole sum cost log-probabilities next to 0 three binary digits (a policy row of 1e-6 relative error, 2e-7 so).
+// Exponentials and their sums are fp32 (a few dozen values per thread, then joined in a fixed order); log q = ln 2 (x c - k) - log(sum) is formed in 64 bits per row, with
 // the logarithm of the sum split into exponent and mantissa: log(sum) rounded to fp32 would alone be off by up to
 // 5e-7, which the ratio of two probabilities and a clip bound next to it would see.
 #include <math.h>
@@ -107,7 +109,7 @@ __device__ __forceinline__ float exp2_approx(float v) {
     return r;
 }
 __device__ __forceinline__ float weight(float x, float k, float c) { return exp2_approx(fmaf(x, c, -k)); }
-__device__ __forceinline__ float reference(float m, float c) { return ceilf(m * c); }
+__device__ __forceinline__ float reference(float m, float c) { return m * c; }
 __device__ __forceinline__ float finite_ref(float k) { return k == -INFINITY ? 0.0f : k; }
 __device__ __forceinline__ float weight4(float4 v, float k, float c) {
     v = make_float4(weight(v.x, k, c), weight(v.y, k, c), weight(v.z, k, c), weight(v.w, k, c));
@@ -694,7 +696,7 @@ row_stream_kernel(const RowParams p, const L loss) {
 
 // ---- rows of any length, loss and statistics alone -------------------------------------------------------
 // A thread keeps a running reference k and sum s over its pieces of the row, four 16-byte loads at a time: the maximum of
-// the sixteen values first, one rescaling of s (a power of two) if it rose, then sixteen exponentials.
+// the sixteen values first, one rescaling of s if it rose, then sixteen exponentials.
 template <class L>
 __global__ void __launch_bounds__(512 + 32)
 row_loss_wide_kernel(const RowParams p, const L loss) {

@@ -80,7 +80,8 @@ def _forward(torch, vm, d, m, k, f, act, save=True, alpha=None, stream=None):
 
 
 SHAPES = [(1, 1, 1), (1, 64, 96), (1, 4096, 128), (1, 257, 65), (2, 512, 130), (3, 1028, 77), (4, 256, 8), (7, 100, 33),
-          (8, 1024, 64), (15, 2052, 129), (16, 512, 512), (17, 512, 96), (33, 130, 70), (48, 1024, 200), (64, 4096, 64),
+          (8, 1024, 64), (15, 2052, 129), (16, 512, 512), (17, 512, 96), (33, 130, 70), (24, 68, 9), (25, 4100, 61),
+          (32, 1028, 33), (41, 260, 500), (48, 1024, 200), (64, 4096, 64),
           (100, 96, 300), (129, 257, 255), (391, 512, 1365), (256, 512, 1024), (2048, 64, 64), (300, 1000, 700),
           (1024, 1024, 1024), (1153, 2048, 640), (5, 3, 4096), (640, 2056, 515), (300, 1000, 1100), (300, 1001, 1100),
           (1290, 520, 1030), (1280, 4104, 1024), (4104, 256, 520)]
@@ -105,7 +106,7 @@ def test_forward_and_gradients(torch_cuda, vm, shape):
 
 
 @pytest.mark.parametrize("path", ["warp", "planes", "raw"])
-@pytest.mark.parametrize("shape", [(17, 33, 35), (20, 64, 32), (33, 132, 70), (100, 96, 300), (129, 257, 255), (200, 300, 130), (700, 40, 48)])
+@pytest.mark.parametrize("shape", [(17, 33, 35), (49, 64, 32), (33, 131, 70), (60, 132, 70), (100, 96, 300), (129, 257, 255), (200, 300, 130), (700, 40, 48)])
 def test_every_kernel_at_odd_sizes(torch_cuda, pkg, vm, shape, path):
     """The sizes at which the dispatch changes kernels, moved out of the way."""
     torch = torch_cuda
