@@ -401,8 +401,8 @@ struct Policy {
         Result out;
         out.loss = free ? -ra : -ba;
         out.slope = free ? -ra : 0.0f;
-        if (ref_logp != nullptr && beta != nullptr) {
-            const float b = __ldg(beta);
+        const float b = (ref_logp != nullptr && beta != nullptr) ? __ldg(beta) : 0.0f;
+        if (b != 0.0f) {          // a coefficient of 0 is no term, even where e^d has overflowed
             const float d = static_cast<float>(static_cast<double>(v.ref) - l);
             const float e1 = expm1f(d);          // e^d - 1: the term is d^2 / 2 next to 0, e^d - d - 1 would cancel
             out.loss = fmaf(b, e1 - d, out.loss);

@@ -290,6 +290,35 @@ def test_policy_rows_and_bounds(torch_cuda, vm, mode):
         _near(a, w, tol)
 
 
+def test_policy_without_a_coefficient_ignores_the_reference(torch_cuda, vm):
+    n, c = 4, 64
+    x, z, old, ref, adv, gy = _policy_inputs(n, c, 1.0, 8)
+    ref[1] = 1e5                                  # e^d overflows
+    for mode in ("step", "calls"):
+        got = _run_policy(torch_cuda, vm, mode, x, z, old, ref, adv, 1.0, gy, beta=0.0)
+        want = _policy_truth(x, z, old, None, adv, 1.0, gy, 0.2, 0.3, 0.0)
+        for a, w, tol in zip(got, want[:3], want[3:]):
+            _near(a, w, tol)
+
+
+def test_more_logits_than_32_bits_count(torch_cuda, vm):
+    """2.2e9 logits, gradient in place: the last rows land where they belong."""
+    torch = torch_cuda
+    n, c = 66000, 32771
+    x = torch.zeros((n, c), device="cuda")
+    z = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    adv, y = torch.ones(n, device="cuda"), torch.empty(n, device="cuda")
+    rows = [0, 32768, n - 2, n - 1]
+    z[rows] = torch.tensor([5, 6, c - 1, 0], dtype=torch.int32, device="cuda")
+    x[rows, :3] = torch.tensor([1.0, -2.0, 3.0], device="cuda")
+    head = x[rows].cpu().numpy()
+    vm.softmax_policy_loss_step(0, y, None, x, None, x, z, None, None, adv, n, c)
+    torch.cuda.synchronize()
+    want = _policy_truth(head, z[rows].cpu().numpy(), None, None, np.ones(4, np.float32), 1.0, np.ones(4, np.float32), np.inf, np.inf, 0.0)
+    _near(to_host(x[rows]), want[2], want[5])
+    assert float(x[1:1000].abs().max()) == 0.0 and float(x[n - 1000: n - 2].abs().max()) == 0.0
+
+
 def test_policy_gradient_against_differences(torch_cuda, vm):
     """The loss is of size 1, off by 2e-6; h = 0.02, third derivative below 2: 2e-6 / 0.02 + 0.0004 / 3 < 3e-4."""
     c, h = 30, 0.02
