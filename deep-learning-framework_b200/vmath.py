@@ -16,13 +16,14 @@ from . import capi
 def _ptr(x):
     if x is None or type(x) is int:        # ctypes turns integers into pointers
         return x
-    if hasattr(x, "data_ptr"):
-        if not x.is_contiguous():
-            raise ValueError("tensor arguments must be contiguous (the reference has no strides)")
-        return x.data_ptr()
-    if isinstance(x, int):
-        return int(x)
-    raise TypeError(f"cannot take the address of {type(x)!r}")
+    try:
+        if x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        if isinstance(x, int):
+            return int(x)
+        raise TypeError(f"cannot take the address of {type(x)!r}") from None
+    raise ValueError("tensor arguments must be contiguous (the reference has no strides)")
 
 
 _type_names = {}     # torch.dtype -> its text, which torch puts together anew on every call
@@ -33,7 +34,10 @@ def _typed(x, name):
     if x is None or type(x) is int:
         return x
     kind = getattr(x, "dtype", None)
-    if kind is not None and _type_names.setdefault(kind, str(kind)) != name:
+    text = _type_names.get(kind)
+    if text is None and kind is not None:
+        text = _type_names[kind] = str(kind)
+    if text != name and kind is not None:
         raise TypeError(f"a tensor of {name} is needed here, got {kind}")
     return _ptr(x)
 
