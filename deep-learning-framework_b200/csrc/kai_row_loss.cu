@@ -27,6 +27,10 @@
 // for its load, 3500 in the two passes, 3500 to 5000 at the cluster barrier, 2000 to 2700 for statistics and slope, 3000 for the
 // gradient, 2500 until the store has read its source), with 34 to 39 % of the issue slots used: it is bound by the latency of that
 // chain.  Measured without gain: parts of 4096 to 16384 columns, 64 to 256 threads, cluster sizes between the powers of two.
+// row_short_kernel takes rows of up to 2048 columns with up to 256 labels, a warp each: there the barriers and the label warp of
+// row_stream_kernel cost more than the row.  Loss and gradient of 8192 rows, the stream's time first: 97 columns, 64 labels 37 us and
+// 14.5; 1000 columns, 256 labels 155 and 40 (64 labels: 44 and 23); 2000 columns, 200 labels 123 and 52; policy loss, 8191 x 1000 29
+// and 17.5 (10 at the copy rate; bound by the chain of one row in the 24 warps per SM that its registers leave).
 // row_loss_wide_kernel takes the rows that the shared memory of a cluster cannot hold (more than 400000 columns), for kLoss;
 // kStep is then kLoss and kGrad.
 //
@@ -55,7 +59,7 @@ enum : int { kLive = 0, kPadding = 1, kBad = 2 };
 
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr int kMaxParts = 8;
-constexpr int kMaxWarps = 16;
+constexpr int kShortWarps = 4;
 
 // ---- row geometry ----------------------------------------------------------------------------------
 // A row of any length at any 4-byte alignment is `head` scalars up to a 16-byte boundary, `quads` 16-byte pieces, and the
@@ -139,6 +143,7 @@ struct alignas(16) RowHead {
     float stat[3];           // the saved row of ps (kGrad): reference, sum, slope
     int state;
     float teacher, weights;  // distillation: reference and sum of the teacher's weights
+    int lone;                // distillation: no id occurs twice
 };
 constexpr int kParked = 8;  // rows whose losses are settled together
 static_assert(sizeof(RowHead) % 16 == 0, "what follows it in shared memory is read 16 bytes at a time");
@@ -164,15 +169,19 @@ struct Distill {
     const int* idx;
     const float* t;
     int ntop, ntop4;       // ntop4: rounded up to a multiple of 4, unused entries behind ntop
+    int bits;              // log2 of the 16-bit places that `merged` has room for
 
     struct Row : RowHead {};
+    // row_short_kernel has room for a table of its own, four to eight places for a label (row_stream_kernel: 512 bytes more would
+    // cost it a CTA per SM at 8000 columns, 98 us becoming 106).
+    __host__ __device__ size_t table_bytes() const { return size_t(2) << (bits + 2); }
     __host__ __device__ size_t bytes() const { return sizeof(RowHead) + 20 * static_cast<size_t>(ntop4); }
     static __device__ __forceinline__ int* ids(Row* r) { return reinterpret_cast<int*>(r + 1); }
     __device__ __forceinline__ float* probs(Row* r) const { return reinterpret_cast<float*>(ids(r) + ntop4); }
     __device__ __forceinline__ float* logits(Row* r) const { return probs(r) + ntop4; }
     __device__ __forceinline__ float* teacher(Row* r) const { return logits(r) + ntop4; }
     __device__ __forceinline__ float* merged(Row* r) const { return teacher(r) + ntop4; }
-    __device__ __forceinline__ int labels() const { return ntop; }
+    __host__ __device__ __forceinline__ int labels() const { return ntop; }
 
     // The label warp works ahead so that no load of its own is waited for: ids and teacher logits are fetched two rows ahead
     // (Ahead), the student's logits there one row ahead (Flight), up to kAhead labels per lane; what is beyond is loaded in
@@ -202,10 +211,38 @@ struct Distill {
             f.x[i] = (z >= 0 && z < ncol && (all || shape.owned(z, part))) ? x[z] : 0.0f;
         }
     }
+    // Whether no id of the row is repeated, by one warp.  Each label writes its place into a table of any content, where a hash of
+    // its id says, and reads back who stands there: itself, and it is done; the same id, and there is a repetition;
+    // another id, and it tries again without those that are done.  Labels of one id that both lost try again together.  Every try
+    // settles one label for each place in use, so tries end.  Against a search for each label, loss and gradient: 2048 x 32000
+    // with 256 labels 227 us and 146, with 1000 labels 2115 and 505; 8192 x 2500 with 64 labels 68 and 58.5.
+    __device__ __forceinline__ bool distinct(const int* id, uint16_t* table, int log) const {
+        const int lane = threadIdx.x & 31;
+        uint64_t open = 0;                     // of the labels lane + 32 i (KAI_TOP_MAX: 64 of them)
+        for (int i = 0, j = lane; j < ntop; ++i, j += 32)
+            if (id[j] >= 0) open |= uint64_t(1) << i;
+        bool twice = false;
+        while (__any_sync(0xffffffffu, open != 0)) {
+            for (int i = 0, j = lane; j < ntop; ++i, j += 32)
+                if (open >> i & 1) table[place(id[j], log)] = static_cast<uint16_t>(j);
+            __syncwarp();
+            for (int i = 0, j = lane; j < ntop; ++i, j += 32)
+                if (open >> i & 1) {
+                    const int who = table[place(id[j], log)];
+                    if (who == j) open &= ~(uint64_t(1) << i);
+                    else if (id[who] == id[j]) twice = true;
+                }
+            if (__any_sync(0xffffffffu, twice)) return false;
+            __syncwarp();                      // the next try writes where this one has read
+        }
+        return true;
+    }
+    __device__ __forceinline__ uint32_t place(int z, int log) const { return static_cast<uint32_t>(z) * 2654435761u >> (32 - log); }
     // One warp: labels and logits into shared memory, the teacher's entries as probabilities (0 for unused entries), and
     // the row's state.
     __device__ __forceinline__ void arrive(Row* r, const Flight& f, const Ahead& a, const float* x, const RowShape& shape,
-                                           int part, bool all, int64_t row, int64_t ncol, const Temp& tv, bool gradient) const {
+                                           int part, bool all, int64_t row, int64_t ncol, const Temp& tv, bool gradient,
+                                           uint16_t* table) const {
         const int lane = threadIdx.x & 31;
         int* id = ids(r);
         float* p = probs(r);
@@ -245,19 +282,25 @@ struct Distill {
         sum = warp_sum(sum);
         const float inv = some ? 1.0f / sum : 0.0f;
         for (int j = lane; j < ntop4; j += 32) p[j] *= inv;
-        if (gradient && ntop <= kMergeAhead) {
-            // repeated ids: the first place of an id takes the sum, the others are marked
+        bool lone = gradient && !bad;
+        if (gradient) {
             __syncwarp();
-            for (int j = lane; j < ntop; j += 32) {
-                int first = j;
-                float sum_j = 0.0f;
-                if (id[j] >= 0) search(r, id[j], 0, 1, first, sum_j);
-                merged(r)[j] = (id[j] >= 0 && first == j) ? sum_j : -1.0f;
+            if (lone) lone = (table != nullptr) ? distinct(id, table, bits + 2) : distinct(id, reinterpret_cast<uint16_t*>(merged(r)), bits);
+            __syncwarp();
+            if (lone || ntop <= kMergeAhead) {
+                // repeated ids: the first place of an id takes the sum, the others are marked
+                for (int j = lane; j < ntop; j += 32) {
+                    int first = j;
+                    float sum_j = p[j];
+                    if (!lone && id[j] >= 0) { sum_j = 0.0f; search(r, id[j], 0, 1, first, sum_j); }
+                    merged(r)[j] = (id[j] >= 0 && first == j) ? sum_j : -1.0f;
+                }
             }
         }
         if (lane == 0) {
             r->teacher = k;
             r->weights = sum;
+            r->lone = lone;
             r->state = bad ? kBad : (some ? kLive : kPadding);
         }
     }
@@ -293,8 +336,9 @@ struct Distill {
     }
     __device__ __forceinline__ float finish_slope(Row*, float, float, const Temp&) const { return 1.0f; }
     __device__ __forceinline__ float coef(Row* r, float, const Temp& tv) const { return r->gy * tv.t; }
-    // Up to this many labels the label warp joins repeated ids while it waits for the others anyway (as part of the gradient's pass
-    // it cost 3500 clocks per row at 64 labels); beyond, its time would grow with the square, and all threads share it.
+    // Where ids are repeated, up to this many labels the label warp joins them while it waits for the others anyway (as part of the
+    // gradient's pass it cost 3500 clocks per row at 64 labels); beyond, its time would grow with the square, and all threads
+    // share it.
     static constexpr int kMergeAhead = 128;
     // Places of id z: the first of them, and the sum of their probabilities.  Thread `sub` of `g` looks at every g-th group of four.
     __device__ __forceinline__ void search(Row* r, int z, int sub, int g, int& first, float& sum) const {
@@ -313,16 +357,16 @@ struct Distill {
         }
     }
     // Threads that share the search for one label's repetitions, as a power of two (32 at most), `threads` being a multiple of 32.
-    __device__ __forceinline__ int sharers(int threads) const {
+    __device__ __forceinline__ int sharers(const Row* r, int threads) const {
         int g = 0;
-        while (ntop > kMergeAhead && g < 5 && (ntop << (g + 1)) <= threads) ++g;
+        while (!r->lone && ntop > kMergeAhead && g < 5 && (ntop << (g + 1)) <= threads) ++g;
         return g;
     }
     // Label j's column and weight; an id that occurs again belongs to its first place.  Called by whole warps.
     __device__ __forceinline__ bool label(Row* r, int j, int sub, int g, int& c, float& w, float& x) const {
         const int z = j < ntop ? ids(r)[j] : -1;
         c = z;
-        if (ntop <= kMergeAhead) {
+        if (r->lone || ntop <= kMergeAhead) {
             if (z < 0) return false;
             w = merged(r)[j];
             x = logits(r)[j];
@@ -363,12 +407,13 @@ struct Policy {
         float x, old, ref, adv;
     };
 
+    __host__ __device__ size_t table_bytes() const { return 0; }
     struct Row : RowHead {
         Flight token;
         int id;
     };
     __host__ __device__ size_t bytes() const { return sizeof(Row); }
-    __device__ __forceinline__ int labels() const { return 1; }
+    __host__ __device__ __forceinline__ int labels() const { return 1; }
 
     __device__ __forceinline__ void ahead(Ahead& a, int64_t row) const { a.id = z[row]; }
     __device__ __forceinline__ void depart(Flight& f, const Ahead& a, const float* x, const RowShape& shape, int part, bool all,
@@ -379,7 +424,7 @@ struct Policy {
         f.adv = (adv != nullptr) ? adv[row] : 0.0f;
     }
     __device__ __forceinline__ void arrive(Row* r, const Flight& f, const Ahead& a, const float*, const RowShape&, int, bool,
-                                           int64_t, int64_t ncol, const Temp&, bool) const {
+                                           int64_t, int64_t ncol, const Temp&, bool, uint16_t*) const {
         if ((threadIdx.x & 31) == 0) {
             r->id = a.id;
             r->state = (a.id >= 0 && a.id < ncol) ? kLive : (a.id == -1 ? kPadding : kBad);
@@ -418,7 +463,7 @@ struct Policy {
     __device__ __forceinline__ float coef(Row* r, float slope, const Temp& tv) const {
         return -(r->gy * slope) / tv.t;
     }
-    __device__ __forceinline__ int sharers(int) const { return 0; }
+    __device__ __forceinline__ int sharers(const Row*, int) const { return 0; }
     __device__ __forceinline__ bool label(Row* r, int j, int, int, int& c, float& w, float& x) const {
         c = r->id;
         w = 1.0f;
@@ -560,7 +605,7 @@ row_stream_kernel(const RowParams p, const L loss) {
         Row* r = reinterpret_cast<Row*>(rows + buf * row_bytes);
         if (lane == 0) r->gy = gy_next;
         if (MODE == kGrad && lane < 3) r->stat[lane] = ps_next;
-        loss.arrive(r, flight, ids, x, shape, part, MODE != kGrad, row, p.ncol, tv, MODE != kLoss);
+        loss.arrive(r, flight, ids, x, shape, part, MODE != kGrad, row, p.ncol, tv, MODE != kLoss, nullptr);
     };
 
     if (first < p.nrow) {
@@ -655,7 +700,7 @@ row_stream_kernel(const RowParams p, const L loss) {
                 if (loose) loose_sh[tid] = weight(lv, kf, tv.c) * f;
                 asm volatile("bar.sync 1, %0;" ::"n"(T) : "memory");
                 // the labels' columns, over what has just been written there
-                const int g = loss.sharers(T);
+                const int g = loss.sharers(r, T);
                 for (int j0 = 0; j0 < loss.labels(); j0 += T >> g) {
                     const int j = j0 + (tid >> g);
                     int c;
@@ -698,6 +743,90 @@ row_stream_kernel(const RowParams p, const L loss) {
     }
 }
 
+// ---- short rows: a warp each -------------------------------------------------------------------------------
+// A row of up to 32 E columns lies in the registers of one warp, column lane + 32 i in value i: loads and stores of 128 bytes
+// whatever the row's alignment, no barrier beyond the warp, and the label's work between the row's loads and their use.
+template <class L, int E, int MODE>
+__global__ void __launch_bounds__(kShortWarps * 32, E <= 16 ? 8 : E <= 32 ? 6 : 4)
+row_short_kernel(const RowParams p, const L loss) {
+    extern __shared__ __align__(16) uint8_t dyn[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const size_t row_bytes = loss.bytes();
+    typename L::Row* r = reinterpret_cast<typename L::Row*>(dyn + warp * row_bytes);
+    typename L::Parked* parked = reinterpret_cast<typename L::Parked*>(dyn + kShortWarps * row_bytes) + warp;
+    const int ncol = static_cast<int>(p.ncol);
+    uint16_t* table = reinterpret_cast<uint16_t*>(dyn + kShortWarps * (row_bytes + (MODE == kGrad ? 0 : sizeof(typename L::Parked))) +
+                                                  warp * loss.table_bytes());
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kShortWarps + warp, step = static_cast<int64_t>(gridDim.x) * kShortWarps;
+    const Temp tv(p.temp);
+    typename L::Ahead ids;
+    if (first < p.nrow) loss.ahead(ids, first);
+    int waiting = 0;
+    for (int64_t row = first; row < p.nrow; row += step) {
+        const int64_t next = row + step;
+        const float* x = p.x + row * p.ncol;
+        float v[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = (lane + 32 * i < ncol) ? __ldcs(x + lane + 32 * i) : -INFINITY;
+        const RowShape shape(x, ncol, ncol);                 // one part
+        typename L::Flight flight;
+        loss.depart(flight, ids, x, shape, 0, true, row, p.ncol);
+        float k = 0.0f, total = 0.0f, slope = 0.0f;
+        if (MODE == kGrad) { k = p.ps[3 * row]; total = p.ps[3 * row + 1]; slope = p.ps[3 * row + 2]; }
+        if (lane == 0) r->gy = (MODE != kLoss && p.gy != nullptr) ? p.gy[row] : 1.0f;
+        loss.arrive(r, flight, ids, x, shape, 0, true, row, p.ncol, tv, MODE != kLoss, table);
+        if (next < p.nrow) loss.ahead(ids, next);
+        __syncwarp();
+        if (MODE != kGrad) {
+            float m = v[0];
+#pragma unroll
+            for (int i = 1; i < E; ++i) m = fmaxf(m, v[i]);
+            k = reference(warp_max(fmaxf(m, -INFINITY)), tv.c);
+            const float kf = finite_ref(k);
+            float part[4] = {};
+#pragma unroll
+            for (int i = 0; i < E; ++i) part[i & 3] += weight(v[i], kf, tv.c);
+            total = warp_sum((part[0] + part[1]) + (part[2] + part[3]));
+            if (MODE == kStep) slope = loss.finish_slope(r, k, total, tv);
+        }
+        const int state = r->state;
+        if (MODE != kLoss) {
+            const float kf = finite_ref(k);
+            const float coef = loss.coef(r, slope, tv);
+            const float f = coef / total;                                   // gradient = f * 2^(x c - k)
+            float* gx = p.gx + row * p.ncol;
+            if (state == kLive) {
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (lane + 32 * i < ncol) gx[lane + 32 * i] = weight(v[i], kf, tv.c) * f;
+                __syncwarp();
+                // the labels' columns, over what has just been written there
+                for (int j0 = 0; j0 < loss.labels(); j0 += 32) {
+                    int c;
+                    float w, xv;
+                    if (loss.label(r, j0 + lane, 0, 1, c, w, xv)) gx[c] = weight(xv, kf, tv.c) * f - coef * w;
+                }
+            } else {
+                // a padding row's logits are not looked at; a bad label poisons the row
+                const float fixed = state == kPadding ? 0.0f : nanf("");
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (lane + 32 * i < ncol) gx[lane + 32 * i] = fixed;
+            }
+        }
+        if (MODE != kGrad) {
+            loss.park(parked, waiting, r, k, total, tv);
+            if (++waiting == kParked || next >= p.nrow) {
+                settle_rows(p, loss, parked, waiting, row - (waiting - 1) * step, step, tv);
+                waiting = 0;
+            }
+        } else if (lane == 0 && state == kBad) {
+            *p.flag = 1;
+        }
+        __syncwarp();                                        // the label buffer is filled again
+    }
+}
+
 // ---- rows of any length, loss and statistics alone -------------------------------------------------------
 // A thread keeps a running reference k and sum s over its pieces of the row, four 16-byte loads at a time: the maximum of
 // the sixteen values first, one rescaling of s if it rose, then sixteen exponentials.
@@ -722,7 +851,7 @@ row_loss_wide_kernel(const RowParams p, const L loss) {
             typename L::Flight flight;
             loss.ahead(ids, row);
             loss.depart(flight, ids, x, shape, part, true, row, p.ncol);
-            loss.arrive(r, flight, ids, x, shape, part, true, row, p.ncol, tv, false);
+            loss.arrive(r, flight, ids, x, shape, part, true, row, p.ncol, tv, false, nullptr);
         }
     } else {
         const float4* xq = reinterpret_cast<const float4*>(x + shape.head);
@@ -769,6 +898,8 @@ row_loss_wide_kernel(const RowParams p, const L loss) {
 // ---- host side -----------------------------------------------------------------------------------------------
 constexpr int64_t kPart = 12800;      // columns of a part at most, where a row has several: 50 KB, four parts to an SM
 constexpr int64_t kPartOne = 16384;   // columns from which on a part is a matter for 256 threads
+constexpr int64_t kShort = 2048;      // columns that a warp takes by itself, with kShortLabels labels at most
+constexpr int kShortLabels = 256;
 constexpr size_t kSmemMost = 220 * 1024;
 
 // Clusters (or, for `parts` = 1, CTAs) of a kernel that are resident on the device at once: the size of a persistent grid.
@@ -873,7 +1004,8 @@ int row_parts(int64_t nrow, int64_t ncol, int64_t most, int sm_count) {
     return static_cast<int>(parts);
 }
 
-// Threads of a CTA: 64 for many short rows (a part of 2048 columns at most), 256 for parts beyond kPartOne and where there are too
+// Threads of a CTA: 64 for many short rows (a part of 2048 columns at most; those with more labels than row_short_kernel takes: 8192 x
+// 250, 200 labels, loss 29 us, with 128 threads 43), 256 for parts beyond kPartOne and where there are too
 // few parts to give every SM four, 128 otherwise.
 template <class L, int MODE>
 int launch_threads(DeviceState* st, const RowParams& p, const L& loss, cudaStream_t s) {
@@ -883,9 +1015,31 @@ int launch_threads(DeviceState* st, const RowParams& p, const L& loss, cudaStrea
     return launch_stream<L, 128, MODE>(st, p, loss, s);
 }
 
+// Rows that lie in a warp's registers.
+template <class L, int E, int MODE>
+int launch_short(DeviceState* st, const RowParams& p, const L& loss, cudaStream_t s) {
+    auto kernel = row_short_kernel<L, E, MODE>;
+    const size_t smem = kShortWarps * (loss.bytes() + (MODE == kGrad ? 0 : sizeof(typename L::Parked)) + (MODE == kLoss ? 0 : loss.table_bytes()));
+    int blocks = 0;
+    KAI_TRY(resident_clusters(reinterpret_cast<const void*>(kernel), kShortWarps * 32, 1, smem, st->sm_count, &blocks));
+    const int64_t groups = (p.nrow + kShortWarps - 1) / kShortWarps;
+    return launch_rows(kernel, "row_short_kernel", p, loss, groups < blocks ? groups : blocks, kShortWarps * 32, false, smem, s);
+}
+template <class L>
+bool takes_short(const RowParams& p, const L& loss) { return p.ncol <= kShort && loss.labels() <= kShortLabels; }
+template <class L, int MODE>
+int run_short(DeviceState* st, RowParams p, L loss, cudaStream_t s) {
+    p.parts = 1;
+    if (p.ncol <= 256) return launch_short<L, 8, MODE>(st, p, loss, s);
+    if (p.ncol <= 512) return launch_short<L, 16, MODE>(st, p, loss, s);
+    if (p.ncol <= 1024) return launch_short<L, 32, MODE>(st, p, loss, s);
+    return launch_short<L, 64, MODE>(st, p, loss, s);
+}
+
 template <class L>
 int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
+    if (takes_short(p, loss)) return run_short<L, kGrad>(st, p, loss, s);
     p.parts = row_parts(p.nrow, p.ncol, int64_t(1) << 20, st->sm_count);
     return launch_threads<L, kGrad>(st, p, loss, s);
 }
@@ -893,6 +1047,7 @@ int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
 template <class L, int MODE>
 int run_rows(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
+    if (takes_short(p, loss)) return run_short<L, MODE>(st, p, loss, s);
     if (stream_smem<L, MODE>(p.ncol, kMaxParts, loss) > kSmemMost) {
         if (MODE == kLoss) return run_wide(st, p, loss, s);
         KAI_TRY(ensure_aux(st, p.nrow * 3 * 4));
@@ -914,7 +1069,10 @@ RowParams row_params(const float* x, int64_t nrow, int64_t ncol, const float* te
     return p;
 }
 Distill distill(const int* idx, const float* t, int64_t ntop) {
-    return Distill{idx, t, static_cast<int>(ntop), static_cast<int>((ntop + 3) / 4 * 4)};
+    const int ntop4 = static_cast<int>((ntop + 3) / 4 * 4);
+    int bits = 3;
+    while ((2 << bits) <= 2 * ntop4) ++bits;
+    return Distill{idx, t, static_cast<int>(ntop), ntop4, bits};
 }
 
 }  // namespace

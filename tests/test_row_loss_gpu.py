@@ -404,3 +404,94 @@ def test_rows_behind_the_last_keep_their_values(torch_cuda, vm):
     vm.softmax_top_distill_step(0, y, gx, None, x, idx, t, 0, c, k)
     torch.cuda.synchronize()
     assert float(y[n]) == 5.0 and bool((gx[n] == 5.0).all())
+
+
+# Sizes on both sides of what a warp's registers hold, label counts on both sides of what one warp joins.
+@pytest.mark.parametrize("mode", ["step", "calls"])
+@pytest.mark.parametrize("shape", [(37, 256, 9), (21, 257, 64), (19, 512, 130), (23, 513, 33), (17, 1024, 256), (15, 1025, 257), (13, 2048, 128),
+                                   (11, 2049, 129), (9, 2047, 700), (2500, 70, 300), (640, 2500, 40)])
+def test_distill_repeats_at_every_size(torch_cuda, vm, shape, mode):
+    """Rows with repeated ids, with distinct ones and with gaps next to one another, whatever kernel takes them."""
+    n, c, k = shape
+    rng = np.random.default_rng(n + c + k)
+    x = (2.5 * rng.standard_normal((n, c))).astype(np.float32)
+    idx, t = _table(rng, n, c, k, repeat=True)
+    for r in range(0, n, 3):
+        m = min(k, c)
+        idx[r, :m], idx[r, m:] = rng.permutation(c)[:m], -1
+    idx[1::3][rng.random(idx[1::3].shape) < 0.3] = -1
+    temp = 2.0 if c % 2 else 1.0
+    gy = rng.standard_normal(n).astype(np.float32)
+    y, gx, ty, tg = _distill_truth(x, idx, t, temp, gy)
+    for off in (0, 1):
+        got = _run_distill(torch_cuda, vm, mode, x, idx, t, temp, gy, off)
+        _near(got[0], y, ty)
+        _near(got[1], gx, tg)
+
+
+@pytest.mark.parametrize("mode", ["step", "calls"])
+@pytest.mark.parametrize("ncol", [2048, 128256])
+def test_distill_ids_that_a_hash_puts_together(torch_cuda, vm, mode, ncol):
+    """Distinct ids with the same leading bits of a multiplicative hash, alone and with one of them repeated."""
+    z = np.arange(ncol, dtype=np.uint64)
+    near = z[(z * 2654435761 % 2 ** 32) < 2 ** 32 * 24 // ncol].astype(np.int32)
+    n, k = 4, len(near) + 1
+    assert k >= 16
+    rng = np.random.default_rng(ncol)
+    x = (2 * rng.standard_normal((n, ncol))).astype(np.float32)
+    _, t = _table(rng, n, ncol, k)
+    idx = np.stack([np.append(near, -1), np.append(near, near[0]), np.append(near, near[-1])[::-1], np.append(near[::-1], near[3])]).astype(np.int32)
+    gy = rng.standard_normal(n).astype(np.float32)
+    y, gx, ty, tg = _distill_truth(x, idx, t, 1.0, gy)
+    got = _run_distill(torch_cuda, vm, mode, x, idx, t, 1.0, gy)
+    _near(got[0], y, ty)
+    _near(got[1], gx, tg)
+
+
+def test_distill_more_rows_than_warps(torch_cuda, vm):
+    n, c, k = 41003, 5, 3
+    rng = np.random.default_rng(n)
+    x = (2 * rng.standard_normal((n, c))).astype(np.float32)
+    idx, t = rng.integers(-1, c, (n, k)).astype(np.int32), rng.standard_normal((n, k)).astype(np.float32)
+    gy = rng.standard_normal(n).astype(np.float32)
+    y, gx, ty, tg = _distill_truth(x, idx, t, 1.0, gy)
+    got = _run_distill(torch_cuda, vm, "step", x, idx, t, 1.0, gy)
+    _near(got[0], y, ty)
+    _near(got[1], gx, tg)
+
+
+@pytest.mark.parametrize("mode", ["step", "calls"])
+@pytest.mark.parametrize("shape", [(41003, 9), (70, 256), (61, 257), (51, 512), (41, 513), (33, 1024), (31, 1025), (27, 2048), (25, 2049)])
+def test_policy_at_every_size(torch_cuda, vm, shape, mode):
+    n, c = shape
+    x, z, old, ref, adv, gy = _policy_inputs(n, c, 1.0, n * c)
+    want = _policy_truth(x, z, old, ref, adv, 1.0, gy, 0.2, 0.3, 0.1)
+    z = z.copy()
+    gone = np.arange(n) % 7 == 6
+    z[gone] = -1                                   # padding
+    got = _run_policy(torch_cuda, vm, mode, x, z, old, ref, adv, 1.0, gy)
+    for a, w, tol in zip(got, want[:3], want[3:]):
+        _near(a[~gone], w[~gone], tol[~gone])
+        assert np.all(a[gone] == 0.0)
+
+
+@pytest.mark.parametrize("ncol", [300, 1500])
+def test_short_rows_with_bad_labels_keep_their_neighbours(torch_cuda, pkg, vm, ncol):
+    """One bad id among many labels and rows: that row is NaN, all others are as without it."""
+    torch = torch_cuda
+    rng = np.random.default_rng(ncol)
+    n, k = 45, 200
+    x = rng.standard_normal((n, ncol)).astype(np.float32)
+    idx, t = _table(rng, n, ncol, k)
+    gy = np.ones(n, np.float32)
+    lib = pkg.load()
+    for mode in ("step", "calls"):
+        assert lib.kai_device_status_clear(0) == 0
+        want = _run_distill(torch, vm, mode, x, idx, t, 1.0, gy)
+        worse = idx.copy()
+        worse[20, 150], worse[21, 3] = ncol, -7
+        got = _run_distill(torch, vm, mode, x, worse, t, 1.0, gy)
+        assert lib.kai_device_status(0, None) == pkg.capi.E_OUT_OF_RANGE
+        rest = np.delete(np.arange(n), [20, 21])
+        assert all(np.array_equal(a[rest], b[rest]) and np.isnan(a[20:22]).all() for a, b in zip(got, want))
+    assert lib.kai_device_status_clear(0) == 0
