@@ -27,7 +27,7 @@
 // for its load, 3500 in the two passes, 3500 to 5000 at the cluster barrier, 2000 to 2700 for statistics and slope, 3000 for the
 // gradient, 2500 until the store has read its source), with 34 to 39 % of the issue slots used: it is bound by the latency of that
 // chain.  Measured without gain: parts of 4096 to 16384 columns, 64 to 256 threads, cluster sizes between the powers of two.
-// row_short_kernel takes rows of up to 2048 columns with up to 256 labels, a warp each: there the barriers and the label warp of
+// row_short_kernel takes rows of up to 4096 columns (kGrad: 2048) with up to 256 labels, a warp each: there the barriers and the label warp of
 // row_stream_kernel cost more than the row.  Loss and gradient of 8192 rows, the stream's time first: 97 columns, 64 labels 37 us and
 // 14.5; 1000 columns, 256 labels 155 and 40 (64 labels: 44 and 23); 2000 columns, 200 labels 123 and 52; policy loss, 8191 x 1000 29
 // and 17.5 (10 at the copy rate; bound by the chain of one row in the 24 warps per SM that its registers leave).
@@ -285,7 +285,8 @@ struct Distill {
         bool lone = gradient && !bad;
         if (gradient) {
             __syncwarp();
-            if (lone) lone = (table != nullptr) ? distinct(id, table, bits + 2) : distinct(id, reinterpret_cast<uint16_t*>(merged(r)), bits);
+            if (lone)
+                lone = (table != nullptr) ? distinct(id, table, bits + 2) : distinct(id, reinterpret_cast<uint16_t*>(merged(r)), bits);
             __syncwarp();
             if (lone || ntop <= kMergeAhead) {
                 // repeated ids: the first place of an id takes the sum, the others are marked
@@ -747,7 +748,7 @@ row_stream_kernel(const RowParams p, const L loss) {
 // A row of up to 32 E columns lies in the registers of one warp, column lane + 32 i in value i: loads and stores of 128 bytes
 // whatever the row's alignment, no barrier beyond the warp, and the label's work between the row's loads and their use.
 template <class L, int E, int MODE>
-__global__ void __launch_bounds__(kShortWarps * 32, E <= 16 ? 8 : E <= 32 ? 6 : 4)
+__global__ void __launch_bounds__(kShortWarps * 32, E <= 16 ? 8 : E <= 32 ? 6 : E <= 64 ? 4 : 3)
 row_short_kernel(const RowParams p, const L loss) {
     extern __shared__ __align__(16) uint8_t dyn[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -898,7 +899,10 @@ row_loss_wide_kernel(const RowParams p, const L loss) {
 // ---- host side -----------------------------------------------------------------------------------------------
 constexpr int64_t kPart = 12800;      // columns of a part at most, where a row has several: 50 KB, four parts to an SM
 constexpr int64_t kPartOne = 16384;   // columns from which on a part is a matter for 256 threads
-constexpr int64_t kShort = 2048;      // columns that a warp takes by itself, with kShortLabels labels at most
+// Columns that a warp takes by itself, with kShortLabels labels at most.  Beyond 2048 kGrad alone loses by it (8192 x 4090, 64 labels: 56 us
+// in the stream, 66), while loss and gradient in one still gain where the labels are few or many (policy, 8192 x 2500: 47 us
+// and 40, 8192 x 4090: 60 and 54; 64 labels 58 and 56, 69 and 71; 200 labels, 8192 x 2500: 105 and 77).
+constexpr int64_t kShort = 4096, kShortGrad = 2048;
 constexpr int kShortLabels = 256;
 constexpr size_t kSmemMost = 220 * 1024;
 
@@ -1019,27 +1023,32 @@ int launch_threads(DeviceState* st, const RowParams& p, const L& loss, cudaStrea
 template <class L, int E, int MODE>
 int launch_short(DeviceState* st, const RowParams& p, const L& loss, cudaStream_t s) {
     auto kernel = row_short_kernel<L, E, MODE>;
-    const size_t smem = kShortWarps * (loss.bytes() + (MODE == kGrad ? 0 : sizeof(typename L::Parked)) + (MODE == kLoss ? 0 : loss.table_bytes()));
+    const size_t smem = kShortWarps * (loss.bytes() + (MODE == kGrad ? 0 : sizeof(typename L::Parked)) +
+                                       (MODE == kLoss ? 0 : loss.table_bytes()));
     int blocks = 0;
     KAI_TRY(resident_clusters(reinterpret_cast<const void*>(kernel), kShortWarps * 32, 1, smem, st->sm_count, &blocks));
     const int64_t groups = (p.nrow + kShortWarps - 1) / kShortWarps;
     return launch_rows(kernel, "row_short_kernel", p, loss, groups < blocks ? groups : blocks, kShortWarps * 32, false, smem, s);
 }
-template <class L>
-bool takes_short(const RowParams& p, const L& loss) { return p.ncol <= kShort && loss.labels() <= kShortLabels; }
+template <class L, int MODE>
+bool takes_short(const RowParams& p, const L& loss) {
+    return p.ncol <= (MODE == kGrad ? kShortGrad : kShort) && loss.labels() <= kShortLabels;
+}
 template <class L, int MODE>
 int run_short(DeviceState* st, RowParams p, L loss, cudaStream_t s) {
     p.parts = 1;
     if (p.ncol <= 256) return launch_short<L, 8, MODE>(st, p, loss, s);
     if (p.ncol <= 512) return launch_short<L, 16, MODE>(st, p, loss, s);
     if (p.ncol <= 1024) return launch_short<L, 32, MODE>(st, p, loss, s);
+    if constexpr (MODE != kGrad)
+        if (p.ncol > 2048) return launch_short<L, 128, MODE>(st, p, loss, s);
     return launch_short<L, 64, MODE>(st, p, loss, s);
 }
 
 template <class L>
 int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
-    if (takes_short(p, loss)) return run_short<L, kGrad>(st, p, loss, s);
+    if (takes_short<L, kGrad>(p, loss)) return run_short<L, kGrad>(st, p, loss, s);
     p.parts = row_parts(p.nrow, p.ncol, int64_t(1) << 20, st->sm_count);
     return launch_threads<L, kGrad>(st, p, loss, s);
 }
@@ -1047,7 +1056,7 @@ int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
 template <class L, int MODE>
 int run_rows(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
-    if (takes_short(p, loss)) return run_short<L, MODE>(st, p, loss, s);
+    if (takes_short<L, MODE>(p, loss)) return run_short<L, MODE>(st, p, loss, s);
     if (stream_smem<L, MODE>(p.ncol, kMaxParts, loss) > kSmemMost) {
         if (MODE == kLoss) return run_wide(st, p, loss, s);
         KAI_TRY(ensure_aux(st, p.nrow * 3 * 4));

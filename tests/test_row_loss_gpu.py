@@ -409,7 +409,7 @@ def test_rows_behind_the_last_keep_their_values(torch_cuda, vm):
 # Sizes on both sides of what a warp's registers hold, label counts on both sides of what one warp joins.
 @pytest.mark.parametrize("mode", ["step", "calls"])
 @pytest.mark.parametrize("shape", [(37, 256, 9), (21, 257, 64), (19, 512, 130), (23, 513, 33), (17, 1024, 256), (15, 1025, 257), (13, 2048, 128),
-                                   (11, 2049, 129), (9, 2047, 700), (2500, 70, 300), (640, 2500, 40)])
+                                   (11, 2049, 129), (9, 2047, 700), (2500, 70, 300), (640, 2500, 40), (13, 4096, 70), (11, 4097, 256)])
 def test_distill_repeats_at_every_size(torch_cuda, vm, shape, mode):
     """Rows with repeated ids, with distinct ones and with gaps next to one another, whatever kernel takes them."""
     n, c, k = shape
@@ -461,7 +461,7 @@ def test_distill_more_rows_than_warps(torch_cuda, vm):
 
 
 @pytest.mark.parametrize("mode", ["step", "calls"])
-@pytest.mark.parametrize("shape", [(41003, 9), (70, 256), (61, 257), (51, 512), (41, 513), (33, 1024), (31, 1025), (27, 2048), (25, 2049)])
+@pytest.mark.parametrize("shape", [(41003, 9), (70, 256), (61, 257), (51, 512), (41, 513), (33, 1024), (31, 1025), (27, 2048), (25, 2049), (14, 4096)])
 def test_policy_at_every_size(torch_cuda, vm, shape, mode):
     n, c = shape
     x, z, old, ref, adv, gy = _policy_inputs(n, c, 1.0, n * c)
