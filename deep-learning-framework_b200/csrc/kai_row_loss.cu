@@ -27,7 +27,7 @@
 // for its load, 3500 in the two passes, 3500 to 5000 at the cluster barrier, 2000 to 2700 for statistics and slope, 3000 for the
 // gradient, 2500 until the store has read its source), with 34 to 39 % of the issue slots used: it is bound by the latency of that
 // chain.  Measured without gain: parts of 4096 to 16384 columns, 64 to 256 threads, cluster sizes between the powers of two.
-// row_short_kernel takes rows of up to 4096 columns (kGrad: 2048) with up to 256 labels, a warp each: there the barriers and the label warp of
+// row_short_kernel takes rows of up to 4096 columns (kGrad with many rows: 2048) with up to 256 labels, a warp each: there the barriers and the label warp of
 // row_stream_kernel cost more than the row.  Loss and gradient of 8192 rows, the stream's time first: 97 columns, 64 labels 37 us and
 // 14.5; 1000 columns, 256 labels 155 and 40 (64 labels: 44 and 23); 2000 columns, 200 labels 123 and 52; policy loss, 8191 x 1000 29
 // and 17.5 (10 at the copy rate; bound by the chain of one row in the 24 warps per SM that its registers leave).
@@ -899,8 +899,8 @@ row_loss_wide_kernel(const RowParams p, const L loss) {
 // ---- host side -----------------------------------------------------------------------------------------------
 constexpr int64_t kPart = 12800;      // columns of a part at most, where a row has several: 50 KB, four parts to an SM
 constexpr int64_t kPartOne = 16384;   // columns from which on a part is a matter for 256 threads
-// Columns that a warp takes by itself, with kShortLabels labels at most.  Beyond 2048 kGrad alone loses by it (8192 x 4090, 64 labels: 56 us
-// in the stream, 66), while loss and gradient in one still gain where the labels are few or many (policy, 8192 x 2500: 47 us
+// Columns that a warp takes by itself, with kShortLabels labels at most.  Beyond 2048 kGrad alone loses by it where warps have several
+// rows (8192 x 4090, 64 labels: 56 us in the stream, 66; 1000 x 4000, both calls: 23 us and 19), while loss and gradient in one still gain where the labels are few or many (policy, 8192 x 2500: 47 us
 // and 40, 8192 x 4090: 60 and 54; 64 labels 58 and 56, 69 and 71; 200 labels, 8192 x 2500: 105 and 77).
 constexpr int64_t kShort = 4096, kShortGrad = 2048;
 constexpr int kShortLabels = 256;
@@ -1031,8 +1031,9 @@ int launch_short(DeviceState* st, const RowParams& p, const L& loss, cudaStream_
     return launch_rows(kernel, "row_short_kernel", p, loss, groups < blocks ? groups : blocks, kShortWarps * 32, false, smem, s);
 }
 template <class L, int MODE>
-bool takes_short(const RowParams& p, const L& loss) {
-    return p.ncol <= (MODE == kGrad ? kShortGrad : kShort) && loss.labels() <= kShortLabels;
+bool takes_short(const RowParams& p, const L& loss, int sm_count) {
+    const bool several = p.nrow > 3 * kShortWarps * static_cast<int64_t>(sm_count);       // at 168 registers
+    return p.ncol <= (MODE == kGrad && several ? kShortGrad : kShort) && loss.labels() <= kShortLabels;
 }
 template <class L, int MODE>
 int run_short(DeviceState* st, RowParams p, L loss, cudaStream_t s) {
@@ -1040,15 +1041,14 @@ int run_short(DeviceState* st, RowParams p, L loss, cudaStream_t s) {
     if (p.ncol <= 256) return launch_short<L, 8, MODE>(st, p, loss, s);
     if (p.ncol <= 512) return launch_short<L, 16, MODE>(st, p, loss, s);
     if (p.ncol <= 1024) return launch_short<L, 32, MODE>(st, p, loss, s);
-    if constexpr (MODE != kGrad)
-        if (p.ncol > 2048) return launch_short<L, 128, MODE>(st, p, loss, s);
-    return launch_short<L, 64, MODE>(st, p, loss, s);
+    if (p.ncol <= 2048) return launch_short<L, 64, MODE>(st, p, loss, s);
+    return launch_short<L, 128, MODE>(st, p, loss, s);
 }
 
 template <class L>
 int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
-    if (takes_short<L, kGrad>(p, loss)) return run_short<L, kGrad>(st, p, loss, s);
+    if (takes_short<L, kGrad>(p, loss, st->sm_count)) return run_short<L, kGrad>(st, p, loss, s);
     p.parts = row_parts(p.nrow, p.ncol, int64_t(1) << 20, st->sm_count);
     return launch_threads<L, kGrad>(st, p, loss, s);
 }
@@ -1056,7 +1056,7 @@ int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
 template <class L, int MODE>
 int run_rows(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
-    if (takes_short<L, MODE>(p, loss)) return run_short<L, MODE>(st, p, loss, s);
+    if (takes_short<L, MODE>(p, loss, st->sm_count)) return run_short<L, MODE>(st, p, loss, s);
     if (stream_smem<L, MODE>(p.ncol, kMaxParts, loss) > kSmemMost) {
         if (MODE == kLoss) return run_wide(st, p, loss, s);
         KAI_TRY(ensure_aux(st, p.nrow * 3 * 4));
