@@ -29,8 +29,8 @@
 // chain.  Measured without gain: parts of 4096 to 16384 columns, 64 to 256 threads, cluster sizes between the powers of two.
 // row_short_kernel takes rows of up to 4096 columns (kGrad with many rows: 2048) with up to 256 labels, a warp each: there the barriers and the label warp of
 // row_stream_kernel cost more than the row.  Loss and gradient of 8192 rows, the stream's time first: 97 columns, 64 labels 37 us and
-// 14.5; 1000 columns, 256 labels 155 and 40 (64 labels: 44 and 23); 2000 columns, 200 labels 123 and 52; policy loss, 8191 x 1000 29
-// and 17.5 (10 at the copy rate; bound by the chain of one row in the 24 warps per SM that its registers leave).
+// 14.5; 1000 columns, 256 labels 155 and 40 (64 labels: 44 and 23); 2000 columns, 200 labels 123 and 50; policy loss, 8191 x 1000 29
+// and 17 (10 at the copy rate; bound by the chain of one row in the 24 warps per SM that its registers leave).
 // row_loss_wide_kernel takes the rows that the shared memory of a cluster cannot hold (more than 400000 columns), for kLoss;
 // kStep is then kLoss and kGrad.
 //
@@ -59,7 +59,7 @@ enum : int { kLive = 0, kPadding = 1, kBad = 2 };
 
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr int kMaxParts = 8;
-constexpr int kShortWarps = 4;
+constexpr int kShortWarps = 4, kShortLeast = 8;
 
 // ---- row geometry ----------------------------------------------------------------------------------
 // A row of any length at any 4-byte alignment is `head` scalars up to a 16-byte boundary, `quads` 16-byte pieces, and the
@@ -746,7 +746,8 @@ row_stream_kernel(const RowParams p, const L loss) {
 
 // ---- short rows: a warp each -------------------------------------------------------------------------------
 // A row of up to 32 E columns lies in the registers of one warp, column lane + 32 i in value i: loads and stores of 128 bytes
-// whatever the row's alignment, no barrier beyond the warp, and the label's work between the row's loads and their use.
+// whatever the row's alignment, no barrier beyond the warp, and the label's work between the row's loads and their use.  Beyond the
+// smallest E a row has more than 16 E columns (run_short), so that half of the values need no bound.
 template <class L, int E, int MODE>
 __global__ void __launch_bounds__(kShortWarps * 32, E <= 16 ? 8 : E <= 32 ? 6 : E <= 64 ? 4 : 3)
 row_short_kernel(const RowParams p, const L loss) {
@@ -758,6 +759,8 @@ row_short_kernel(const RowParams p, const L loss) {
     const int ncol = static_cast<int>(p.ncol);
     uint16_t* table = reinterpret_cast<uint16_t*>(dyn + kShortWarps * (row_bytes + (MODE == kGrad ? 0 : sizeof(typename L::Parked))) +
                                                   warp * loss.table_bytes());
+    const int rest = ncol - lane;
+    auto inside = [&](int i) { return (E > kShortLeast && 2 * i < E) || 32 * i < rest; };
     const int64_t first = static_cast<int64_t>(blockIdx.x) * kShortWarps + warp, step = static_cast<int64_t>(gridDim.x) * kShortWarps;
     const Temp tv(p.temp);
     typename L::Ahead ids;
@@ -768,7 +771,7 @@ row_short_kernel(const RowParams p, const L loss) {
         const float* x = p.x + row * p.ncol;
         float v[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = (lane + 32 * i < ncol) ? __ldcs(x + lane + 32 * i) : -INFINITY;
+        for (int i = 0; i < E; ++i) v[i] = inside(i) ? __ldcs(x + lane + 32 * i) : -INFINITY;
         const RowShape shape(x, ncol, ncol);                 // one part
         typename L::Flight flight;
         loss.depart(flight, ids, x, shape, 0, true, row, p.ncol);
@@ -786,7 +789,10 @@ row_short_kernel(const RowParams p, const L loss) {
             const float kf = finite_ref(k);
             float part[4] = {};
 #pragma unroll
-            for (int i = 0; i < E; ++i) part[i & 3] += weight(v[i], kf, tv.c);
+            for (int i = 0; i < E; ++i) {
+                v[i] = weight(v[i], kf, tv.c);               // all that kStep needs of it from here on
+                part[i & 3] += v[i];
+            }
             total = warp_sum((part[0] + part[1]) + (part[2] + part[3]));
             if (MODE == kStep) slope = loss.finish_slope(r, k, total, tv);
         }
@@ -799,7 +805,7 @@ row_short_kernel(const RowParams p, const L loss) {
             if (state == kLive) {
 #pragma unroll
                 for (int i = 0; i < E; ++i)
-                    if (lane + 32 * i < ncol) gx[lane + 32 * i] = weight(v[i], kf, tv.c) * f;
+                    if (inside(i)) gx[lane + 32 * i] = (MODE == kStep ? v[i] : weight(v[i], kf, tv.c)) * f;
                 __syncwarp();
                 // the labels' columns, over what has just been written there
                 for (int j0 = 0; j0 < loss.labels(); j0 += 32) {
@@ -812,7 +818,7 @@ row_short_kernel(const RowParams p, const L loss) {
                 const float fixed = state == kPadding ? 0.0f : nanf("");
 #pragma unroll
                 for (int i = 0; i < E; ++i)
-                    if (lane + 32 * i < ncol) gx[lane + 32 * i] = fixed;
+                    if (inside(i)) gx[lane + 32 * i] = fixed;
             }
         }
         if (MODE != kGrad) {
@@ -900,8 +906,8 @@ row_loss_wide_kernel(const RowParams p, const L loss) {
 constexpr int64_t kPart = 12800;      // columns of a part at most, where a row has several: 50 KB, four parts to an SM
 constexpr int64_t kPartOne = 16384;   // columns from which on a part is a matter for 256 threads
 // Columns that a warp takes by itself, with kShortLabels labels at most.  Beyond 2048 kGrad alone loses by it where warps have several
-// rows (8192 x 4090, 64 labels: 56 us in the stream, 66; 1000 x 4000, both calls: 23 us and 19), while loss and gradient in one still gain where the labels are few or many (policy, 8192 x 2500: 47 us
-// and 40, 8192 x 4090: 60 and 54; 64 labels 58 and 56, 69 and 71; 200 labels, 8192 x 2500: 105 and 77).
+// rows (8192 x 4090, 64 labels: 56 us in the stream, 66; 1000 x 4000, both calls: 23 us and 19), while loss and gradient in one still gain (policy, 8192 x 2500: 47 us
+// and 39, 8192 x 4090: 60 and 53; 64 labels 58 and 50, 69 and 68; 200 labels, 8192 x 2500: 105 and 67).
 constexpr int64_t kShort = 4096, kShortGrad = 2048;
 constexpr int kShortLabels = 256;
 constexpr size_t kSmemMost = 220 * 1024;
@@ -1038,7 +1044,7 @@ bool takes_short(const RowParams& p, const L& loss, int sm_count) {
 template <class L, int MODE>
 int run_short(DeviceState* st, RowParams p, L loss, cudaStream_t s) {
     p.parts = 1;
-    if (p.ncol <= 256) return launch_short<L, 8, MODE>(st, p, loss, s);
+    if (p.ncol <= 32 * kShortLeast) return launch_short<L, kShortLeast, MODE>(st, p, loss, s);
     if (p.ncol <= 512) return launch_short<L, 16, MODE>(st, p, loss, s);
     if (p.ncol <= 1024) return launch_short<L, 32, MODE>(st, p, loss, s);
     if (p.ncol <= 2048) return launch_short<L, 64, MODE>(st, p, loss, s);
