@@ -432,6 +432,23 @@ struct Policy {
             r->token = f;
         }
     }
+    // e^d - d - 1, from d in 64 bits, d rounded and e1 = expm1f of that.  Next to 0 it is d^2 / 2 and e1 - d the difference of two numbers
+    // that agree to d / 2, which leaves 2^-24 / d of it (4e-4 at d = 1e-4): up to 1 it is d^2 (1/2 + d (1/6 + d/24 + ...)), nine
+    // terms behind the first (what is left out: 4e-9), of which only the sum behind 1/2 is rounded to fp32.  (exp and expm1 in 64 bits
+    // for ratio and term: 8192 x 97, loss alone, 8.4 us instead of 7.4.)
+    static __device__ __forceinline__ double kl_value(double d, float d32, float e1) {
+        if (!(fabsf(d32) <= 1.0f)) return static_cast<double>(e1) - d;
+        float s = 1.0f / 39916800.0f;
+        s = fmaf(s, d32, 1.0f / 3628800.0f);
+        s = fmaf(s, d32, 1.0f / 362880.0f);
+        s = fmaf(s, d32, 1.0f / 40320.0f);
+        s = fmaf(s, d32, 1.0f / 5040.0f);
+        s = fmaf(s, d32, 1.0f / 720.0f);
+        s = fmaf(s, d32, 1.0f / 120.0f);
+        s = fmaf(s, d32, 1.0f / 24.0f);
+        s = fmaf(s, d32, 1.0f / 6.0f);
+        return d * d * (0.5 + static_cast<double>(s * d32));
+    }
     __device__ __forceinline__ Result finish(const Flight& v, float k, float total, const Temp& tv) const {
         const double l = kLn2 * tv.exponent(v.x, finite_ref(k)) - log_sum(total);
         const float a = v.adv;
@@ -450,10 +467,8 @@ struct Policy {
         const float b = (ref_logp != nullptr && beta != nullptr) ? __ldg(beta) : 0.0f;
         if (b != 0.0f) {          // a coefficient of 0 is no term, even where e^d has overflowed
             const double d = static_cast<double>(v.ref) - l;
-            const float e1 = expm1f(static_cast<float>(d));
-            // The value is d^2 / 2 next to 0, the difference of two numbers that agree to d / 2: rounded to fp32 they would leave it
-            // 2^-24 / d of itself (4e-4 measured at d = 1e-4); in 64 bits 1e-10 is left there.
-            out.loss = static_cast<float>(static_cast<double>(out.loss) + static_cast<double>(b) * (expm1(d) - d));
+            const float d32 = static_cast<float>(d), e1 = expm1f(d32);
+            out.loss = static_cast<float>(static_cast<double>(out.loss) + static_cast<double>(b) * kl_value(d, d32, e1));
             out.slope = fmaf(-b, e1, out.slope);
         }
         out.logp = static_cast<float>(l);
