@@ -52,3 +52,20 @@ def test_kl_term_next_to_the_reference(torch_cuda, vm, ncol, mode):
     slope = -np.expm1(d)
     assert np.all(np.abs(other + slope / ncol) <= 7 * HALF * np.abs(slope) / ncol)
     assert np.all(np.abs(at - slope * (1 - 1 / ncol)) <= 8 * HALF * np.abs(slope))
+
+
+@pytest.mark.parametrize("mode", ["step", "calls"])
+@pytest.mark.parametrize("ncol", SIZES)
+def test_ratio(torch_cuda, vm, ncol, mode):
+    """Advantage -1, no bounds, ratios from e^-12 to e^12: the loss is the ratio e^(l - old) itself: expf of the rounded difference (a unit in the last place: 2 u)
+    times 1 plus what the rounding lost (two roundings; the square of 2^-23 left out).  The gradient's columns are it times q
+    (exact) beside the label's, and its difference to that, rounded again, at the label."""
+    n = 16 if ncol > 8192 else 1500
+    l = -np.log2(ncol) * np.log(2.0)
+    old = (l + np.random.default_rng(ncol).uniform(-12, 12, n)).astype(np.float32)
+    rho = np.exp(l - old.astype(np.float64))
+    z = (np.arange(n) * 7 % ncol).astype(np.int32)
+    y, at, other = _run(torch_cuda, vm, mode, n, ncol, z, old, None, -np.ones(n, np.float32), None)
+    assert np.all(np.abs(y - rho) <= 4 * HALF * rho), np.abs(y / rho - 1).max()
+    assert np.all(np.abs(other + rho / ncol) <= 4 * HALF * rho / ncol)
+    assert np.all(np.abs(at - rho * (1 - 1 / ncol)) <= 5 * HALF * rho)
