@@ -521,6 +521,13 @@ __device__ __forceinline__ void push_stat(float2* local, uint32_t rank, float a,
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(a), "f"(b) : "memory");
 }
+// Raises the same shared-memory flag of CTA `rank`.
+__device__ __forceinline__ void push_flag(int* local, uint32_t rank) {
+    const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(local));
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(1) : "memory");
+}
 // `bytes` (a multiple of 16, both addresses on 16-byte boundaries) into shared memory; the barrier is credited as they land.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
@@ -609,6 +616,10 @@ row_stream_kernel(const RowParams p, const L loss) {
             bulk_load(stage, reinterpret_cast<const float4*>(x + shape.head) + shape.begin(part), bytes, smem_u32(&full));
     };
 
+    // A wait ran out in a CTA of this row: from here on its rows have no logits, whatever the barriers' phases say of them.  They become NaN
+    // (padding rows stay 0), and the CTAs keep in step.  Whoever asks behind the row's barrier gets the same answer in all of them.
+    auto lost = [&] { return *static_cast<volatile int*>(&abort_flag) != 0; };
+
     // The label warp's three stages; every part of a row needs all labels' logits (kStep: the policy's slope hangs on them)
     // or its own (kGrad).
     typename L::Ahead ids, ids_next;
@@ -653,7 +664,8 @@ row_stream_kernel(const RowParams p, const L loss) {
         float lv = -INFINITY;
         if (!labels) {
             if (loose) lv = x[shape.loose_col(tid)];
-            mbar_wait(smem_u32(&full), phase, &abort_flag, p.status, 40);
+            if (!mbar_wait(smem_u32(&full), phase, &abort_flag, p.status, 40) && cluster)
+                for (int i = 0; i < p.parts; ++i) push_flag(&abort_flag, i);
             if (MODE != kGrad) {
                 float m = lv;
 #pragma unroll 4
@@ -685,6 +697,7 @@ row_stream_kernel(const RowParams p, const L loss) {
             if (MODE != kGrad && part == 0) {
                 float k, total;
                 join(stat[buf], p.parts * W, k, total);
+                if (lost()) total = nanf("");
                 loss.park(parked, waiting, r, k, total, tv);
                 if (++waiting == kParked || next >= p.nrow) {
                     settle_rows(p, loss, parked, waiting, row - (waiting - 1) * step, step, tv);
@@ -698,7 +711,7 @@ row_stream_kernel(const RowParams p, const L loss) {
                 ids = ids_next;
             }
         } else if (MODE == kLoss) {
-            if (tid == 0 && next < p.nrow) fetch(next);
+            if (tid == 0 && next < p.nrow && !lost()) fetch(next);
         } else {
             float k, total, slope;
             if (MODE == kGrad) {
@@ -745,7 +758,11 @@ row_stream_kernel(const RowParams p, const L loss) {
             asm volatile("bar.sync 1, %0;" ::"n"(T) : "memory");
             if (loose) gx[shape.loose_col(tid)] = loose_sh[tid];
             float* out = gx + shape.head + 4 * shape.begin(part);
-            if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15) == 0) {
+            if (lost()) {
+                // a copy may still land in the stage: what goes out does not come from there, and nothing more is fetched
+                const float fixed = state == kPadding ? 0.0f : nanf("");
+                for (int i = tid; i < 4 * n; i += T) out[i] = fixed;
+            } else if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15) == 0) {
                 if (tid == 0) {
                     if (n > 0) bulk_store(out, stage, static_cast<uint32_t>(n) * 16u);
                     if (next < p.nrow) fetch(next);
@@ -1072,8 +1089,15 @@ int run_short(DeviceState* st, RowParams p, L loss, cudaStream_t s) {
     return launch_short<L, 128, MODE>(st, p, loss, s);
 }
 
+// What every call with bounded waits answers while an expired one has not been cleared.
+int answer(const DeviceState* st) {
+    if (st->status_host[0] != 0)
+        return fail(KAI_E_DEVICE_WAIT, "a device-side wait ran out earlier (where=%d)", st->status_host[1]);
+    return KAI_OK;
+}
+
 template <class L>
-int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
+int launch_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
     if (takes_short<L, kGrad>(p, loss, st->sm_count)) return run_short<L, kGrad>(st, p, loss, s);
     p.parts = row_parts(p.nrow, p.ncol, int64_t(1) << 20, st->sm_count);
@@ -1081,7 +1105,7 @@ int run_grad(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
 }
 
 template <class L, int MODE>
-int run_rows(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
+int launch_any(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
     p.flag = st->flag_dev + 2;
     if (takes_short<L, MODE>(p, loss, st->sm_count)) return run_short<L, MODE>(st, p, loss, s);
     if (stream_smem<L, MODE>(p.ncol, kMaxParts, loss) > kSmemMost) {
@@ -1089,10 +1113,21 @@ int run_rows(DeviceState* st, RowParams p, const L& loss, cudaStream_t s) {
         KAI_TRY(ensure_aux(st, p.nrow * 3 * 4));
         p.ps = static_cast<float*>(st->aux);
         KAI_TRY(run_wide(st, p, loss, s));
-        return run_grad(st, p, loss, s);
+        return launch_grad(st, p, loss, s);
     }
     p.parts = row_parts(p.nrow, p.ncol, kMaxParts, st->sm_count);
     return launch_threads<L, MODE>(st, p, loss, s);
+}
+
+template <class L>
+int run_grad(DeviceState* st, const RowParams& p, const L& loss, cudaStream_t s) {
+    KAI_TRY(launch_grad(st, p, loss, s));
+    return answer(st);
+}
+template <class L, int MODE>
+int run_rows(DeviceState* st, const RowParams& p, const L& loss, cudaStream_t s) {
+    KAI_TRY((launch_any<L, MODE>(st, p, loss, s)));
+    return answer(st);
 }
 
 RowParams row_params(const float* x, int64_t nrow, int64_t ncol, const float* temp) {
