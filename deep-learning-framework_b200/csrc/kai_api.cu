@@ -1481,6 +1481,13 @@ int kai_gated_linear_forward(int device, float* ph, float* pg, float* pu, const 
     if (share_memory(ph, nh, pg, nh) || share_memory(ph, nh, pu, nh) || share_memory(pg, nh, pu, nh) ||
         share_memory(ph, nh, px, ndat * xvec) || share_memory(pg, nh, px, ndat * xvec) || share_memory(pu, nh, px, ndat * xvec))
         return fail(KAI_E_INVALID_ARG, "gated_linear_forward: an output overlaps another output or px");
+    for (const float* out : {ph, pg, pu})
+        for (const float* w : {pwg, pwu})
+            if (share_memory(out, nh, w, yvec * xvec))
+                return fail(KAI_E_INVALID_ARG, "gated_linear_forward: an output overlaps a weight");
+    for (const float* out : {ph, pg, pu})
+        for (const float* b : {pbg, pbu})
+            if (share_memory(out, nh, b, yvec)) return fail(KAI_E_INVALID_ARG, "gated_linear_forward: an output overlaps a bias");
     KAI_ENTER(device);
     if (ndat == 0 || yvec == 0) return KAI_OK;
     const double flops = 4.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
@@ -1512,6 +1519,10 @@ int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float* pgwu, 
         const int64_t n = v == px ? nx : nh;
         clash = clash || share_memory(pgx, nx, v, n) || share_memory(pgwg, nw, v, n) || share_memory(pgwu, nw, v, n);
     }
+    // pgx is formed from the weights while their gradients are written
+    for (const float* w : {pwg, pwu})
+        clash = clash || share_memory(pgwg, nw, w, nw) || share_memory(pgwu, nw, w, nw) || share_memory(pgg, nh, w, nw) ||
+                share_memory(pgu, nh, w, nw);
     if (clash) return fail(KAI_E_INVALID_ARG, "gated_linear_backward: two buffers overlap");
     KAI_ENTER(device);
     const double flops = 4.0 * static_cast<double>(ndat) * static_cast<double>(yvec) * static_cast<double>(xvec);
