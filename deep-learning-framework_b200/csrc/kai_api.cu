@@ -1388,7 +1388,7 @@ static int no_host_path(int device) {
 // Whether two buffers of that many floats share memory without being the same one.
 static bool partly_overlap(const float* a, int64_t na, const float* b, int64_t nb) {
     const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
-    return a != nullptr && b != nullptr && pa != pb && pa < pb + 4 * static_cast<uintptr_t>(nb) &&
+    return a != nullptr && b != nullptr && na > 0 && nb > 0 && pa != pb && pa < pb + 4 * static_cast<uintptr_t>(nb) &&
            pb < pa + 4 * static_cast<uintptr_t>(na);
 }
 // The same, one buffer included.

@@ -33,3 +33,10 @@ def test_gated_outputs_over_weights_and_biases(name, changes):
 def test_gated_neighbours_are_no_overlap():
     _on_the_device("kai_gated_linear_forward", {1: D + 512, 2: E - 128, 3: E + 512, 7: A - 32, 8: A + 128})
     _on_the_device("kai_gated_linear_backward", {2: I + 512, 3: J + 512, 4: I - 128, 5: J - 128})
+
+
+def test_an_empty_operand_lies_nowhere():
+    """Whatever its address: a call without rows is not refused for a pointer that falls into another buffer."""
+    _on_the_device("kai_gated_linear_backward", {1: B + 64, 13: 0})
+    _on_the_device("kai_gated_linear_forward", {1: D + 64, 10: 0})
+    _on_the_device("kai_softmax_top_distill_step", {4: B + 4, 7: 0})
