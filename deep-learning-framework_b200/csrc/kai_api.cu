@@ -1396,6 +1396,28 @@ static bool share_memory(const float* a, int64_t na, const float* b, int64_t nb)
     return partly_overlap(a, na, b, nb) || (a != nullptr && a == b && na > 0 && nb > 0);
 }
 
+// Whether any of `rows` rows of `n` floats at a, lda apart, shares memory with any at b, ldb apart.
+static bool rows_overlap(const float* a, int64_t lda, const float* b, int64_t ldb, int64_t rows, int64_t n) {
+    if (rows <= 0 || n <= 0 || a == nullptr || b == nullptr) return false;
+    const int64_t pa = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a)), pb = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b));
+    const int64_t len = 4 * n, sa = 4 * lda, sb = 4 * ldb;
+    if (pa >= pb + (rows - 1) * sb + len || pb >= pa + (rows - 1) * sa + len) return false;
+    if (sa == sb) {
+        // the rows of b that begin at or in front of a row of a, and those behind it
+        int64_t ahead = (pb - pa) / sa, rest = (pb - pa) % sa;
+        if (rest < 0) { rest += sa; --ahead; }
+        return (rest < len && ahead < rows && -ahead < rows) || (sa - rest < len && ahead + 1 < rows && -(ahead + 1) < rows);
+    }
+    // two strides in one stretch of memory: both lists in order
+    for (int64_t i = 0, j = 0; i < rows && j < rows;) {
+        const int64_t ai = pa + i * sa, bj = pb + j * sb;
+        if (ai < bj + len && bj < ai + len) return true;
+        if (ai < bj) ++i;
+        else ++j;
+    }
+    return false;
+}
+
 // ---- rotary positions -----------------------------------------------------------------------
 static int rotary_call(const char* name, int device, float* py, const float* px, const double* pfreq, const int64_t* ppos,
                        int64_t pos0, int64_t nbat, int64_t ntimes, int64_t nhead, int64_t npiece, int64_t nrot, int layout,
@@ -1416,8 +1438,8 @@ static int rotary_call(const char* name, int device, float* py, const float* px,
         return fail(KAI_E_INVALID_ARG, "%s: null pointer", name);
     if (py == px && ldy != ldx) return fail(KAI_E_INVALID_ARG, "%s: in place with two row strides", name);
     const int64_t nvec = nhead * npiece;
-    if (ldy == nvec && ldx == nvec && partly_overlap(py, nbat * ntimes * nvec, px, nbat * ntimes * nvec))
-        return fail(KAI_E_INVALID_ARG, "%s: output and input overlap without being one buffer", name);
+    if (py != px && rows_overlap(py, ldy, px, ldx, nbat * ntimes, nvec))
+        return fail(KAI_E_INVALID_ARG, "%s: output and input rows overlap without being the same", name);
     KAI_ENTER(device);
     if (nbat * ntimes * nvec == 0) return KAI_OK;
     return rotary(st, py, px, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot, layout, scale, ldy, ldx, backward, s);

@@ -40,3 +40,52 @@ def test_an_empty_operand_lies_nowhere():
     _on_the_device("kai_gated_linear_backward", {1: B + 64, 13: 0})
     _on_the_device("kai_gated_linear_forward", {1: D + 64, 10: 0})
     _on_the_device("kai_softmax_top_distill_step", {4: B + 4, 7: 0})
+
+
+# rotary: 2 x 3 tokens of 4 heads x 8 values; arguments 6 to 9 are nbat, ntimes, nhead, npiece, 13 and 14 the strides of output and input
+@pytest.mark.parametrize("changes", [
+    {2: A + 64, 13: 96, 14: 96},                  # rows of 128 bytes, half a row on
+    {2: A + 96 * 4 - 64, 13: 96, 14: 96},         # half a row in front of the next one
+    {2: A - 64, 13: 96, 14: 96},
+    {2: A + 5 * 96 * 4 + 124, 13: 96, 14: 96},    # the last row's last value
+    {2: A + 3 * 96 * 4, 13: 96, 14: 96},          # whole rows, three on
+    {2: A + 2, 13: 96, 14: 96},
+    {2: A + 128, 13: 96, 14: 64},                 # strides of 384 and 256 bytes
+    {2: A + 300, 13: 64, 14: 32},
+    {2: A + 4, 7: 1, 6: 1, 13: 96, 14: 40},       # one row: strides do not matter
+])
+@pytest.mark.parametrize("name", ["kai_rotary", "kai_rotary_backward"])
+def test_rotary_rows_that_overlap(name, changes):
+    assert _call(name, {10: 6, **changes}) == BAD
+
+
+@pytest.mark.parametrize("changes", [
+    {2: A, 13: 96, 14: 96}, {2: A + 128, 13: 96, 14: 96}, {2: A + 256, 13: 96, 14: 96}, {2: A - 128, 13: 96, 14: 96},
+    {2: A + 6 * 96 * 4, 13: 96, 14: 96}, {2: A + 5 * 96 * 4 + 128, 13: 96, 14: 96},
+    {2: A + 128, 13: 96, 14: 192}, {2: A + 128, 13: 128, 14: 64}, {2: A + 128, 6: 1, 7: 1, 13: 96, 14: 40},
+])
+def test_rotary_rows_that_do_not(changes):
+    _on_the_device("kai_rotary", changes)
+
+
+def test_rotary_rows_against_a_list_of_every_value():
+    """The same answer as from the sets of addresses themselves, for many small strides, shifts and numbers of rows."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses of this test are not to be read")
+    rng = __import__("random").Random(5)
+    seen = set()
+    for _ in range(3000):
+        rows, w = rng.randint(1, 5), rng.randint(1, 4) * 2
+        ldy, ldx = (w + rng.randint(0, 9) for _ in range(2))
+        if rng.random() < 0.5:
+            ldx = ldy
+        shift = rng.randint(-60, 60)
+        if shift == 0:
+            continue
+        y = {i * ldy + c for i in range(rows) for c in range(w)}
+        x = {shift + i * ldx + c for i in range(rows) for c in range(w)}
+        got = _call("kai_rotary", {2: A + 4 * shift, 6: 1, 7: rows, 8: 1, 9: w, 10: w, 13: ldy, 14: ldx})
+        assert (got == BAD) == bool(x & y), (rows, w, ldy, ldx, shift)
+        seen.add((got == BAD, ldx == ldy))
+    assert len(seen) == 4
