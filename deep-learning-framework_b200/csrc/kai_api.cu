@@ -1396,6 +1396,8 @@ static bool share_memory(const float* a, int64_t na, const float* b, int64_t nb)
     return partly_overlap(a, na, b, nb) || (a != nullptr && a == b && na > 0 && nb > 0);
 }
 
+// Whether rows * width floats are more than any memory holds (the products below stay far from 2^63 then).
+static bool beyond_memory(int64_t rows, int64_t width) { return rows > 0 && width > (int64_t(1) << 56) / rows; }
 // Whether any of `rows` rows of `n` floats at a, lda apart, shares memory with any at b, ldb apart.
 static bool rows_overlap(const float* a, int64_t lda, const float* b, int64_t ldb, int64_t rows, int64_t n) {
     if (rows <= 0 || n <= 0 || a == nullptr || b == nullptr) return false;
@@ -1434,10 +1436,11 @@ static int rotary_call(const char* name, int device, float* py, const float* px,
         return fail(KAI_E_TOO_LARGE, "%s: a row has 2^31 values or more", name);
     if (ldy < nhead * npiece || ldx < nhead * npiece)
         return fail(KAI_E_INVALID_ARG, "%s: a row stride is shorter than nhead * npiece", name);
-    if (nbat * ntimes * nhead * npiece > 0 && (!py || !px || (!pfreq && nrot > 0)))
+    const int64_t nvec = nhead * npiece, widest = ldy > ldx ? ldy : ldx;
+    if (nvec > 0 && beyond_memory(nbat * ntimes, widest)) return fail(KAI_E_TOO_LARGE, "%s: more values than memory holds", name);
+    if (nbat * ntimes * nvec > 0 && (!py || !px || (!pfreq && nrot > 0)))
         return fail(KAI_E_INVALID_ARG, "%s: null pointer", name);
     if (py == px && ldy != ldx) return fail(KAI_E_INVALID_ARG, "%s: in place with two row strides", name);
-    const int64_t nvec = nhead * npiece;
     if (py != px && rows_overlap(py, ldy, px, ldx, nbat * ntimes, nvec))
         return fail(KAI_E_INVALID_ARG, "%s: output and input rows overlap without being the same", name);
     KAI_ENTER(device);
@@ -1564,12 +1567,14 @@ static int row_loss_args(const char* name, int64_t nrow, int64_t ncol) {
     if (nrow < 0 || ncol < 0) return fail(KAI_E_INVALID_ARG, "%s: negative extent", name);
     if (ncol >= (int64_t(1) << 31)) return fail(KAI_E_TOO_LARGE, "%s: labels are 32-bit, ncol is not", name);
     if (ncol == 0 && nrow > 0) return fail(KAI_E_INVALID_ARG, "%s: no columns", name);
+    if (beyond_memory(nrow, ncol)) return fail(KAI_E_TOO_LARGE, "%s: more logits than memory holds", name);
     return KAI_OK;
 }
 static int distill_args(const char* name, int64_t nrow, int64_t ncol, int64_t ntop) {
     KAI_TRY(row_loss_args(name, nrow, ncol));
     if (ntop < 0) return fail(KAI_E_INVALID_ARG, "%s: negative extent", name);
     if (ntop > KAI_TOP_MAX) return fail(KAI_E_TOO_LARGE, "%s: ntop=%lld > %d", name, (long long)ntop, KAI_TOP_MAX);
+    if (beyond_memory(nrow, ntop)) return fail(KAI_E_TOO_LARGE, "%s: more labels than memory holds", name);
     return KAI_OK;
 }
 

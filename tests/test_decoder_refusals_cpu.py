@@ -89,3 +89,17 @@ def test_rotary_rows_against_a_list_of_every_value():
         assert (got == BAD) == bool(x & y), (rows, w, ldy, ldx, shift)
         seen.add((got == BAD, ldx == ldy))
     assert len(seen) == 4
+
+
+@pytest.mark.parametrize("name,changes", [
+    # products that come to 0 or below modulo 2^64
+    ("kai_rotary", {6: 1 << 30, 7: 1 << 30, 8: 1, 9: 16}), ("kai_rotary", {6: 1 << 30, 7: 1 << 30, 8: 1, 9: 8}),
+    ("kai_rotary_backward", {6: 1 << 30, 7: 1 << 30, 8: 1, 9: 16, 10: 16}), ("kai_rotary", {6: 1 << 30, 7: 1 << 20, 13: 1 << 40}),
+    ("kai_rotary", {14: 1 << 62}),
+    ("kai_softmax_top_distill", {6: 1 << 62, 7: 4}), ("kai_softmax_top_distill_step", {7: 1 << 33, 8: (1 << 31) - 1}),
+    ("kai_softmax_top_distill_backward_x", {7: 1 << 60, 8: 16}), ("kai_softmax_policy_loss", {9: 1 << 62, 10: 4}),
+    ("kai_softmax_policy_loss_backward_x", {6: 1 << 60, 7: 16}), ("kai_softmax_policy_loss_step", {10: 1 << 62, 11: 1}),
+    ("kai_softmax_top_distill", {6: 1 << 56, 7: 1, 8: 2048}),
+])
+def test_more_bytes_than_addresses(name, changes):
+    assert _call(name, changes) == LARGE
