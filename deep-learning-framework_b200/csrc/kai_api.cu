@@ -3,6 +3,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <map>
 #include <vector>
 
@@ -1578,12 +1579,36 @@ static int distill_args(const char* name, int64_t nrow, int64_t ncol, int64_t nt
     return KAI_OK;
 }
 
+// Buffers of a row loss as n 32-bit values: none of the outputs may share memory with another buffer, but that the gradient (the first
+// output, where there is one) may be the logits (the first input).
+struct Span {
+    const void* at;
+    int64_t n;
+};
+static int loss_buffers(const char* name, std::initializer_list<Span> outs, std::initializer_list<Span> ins, bool gradient) {
+    auto share = [](const Span& a, const Span& b) {
+        return share_memory(static_cast<const float*>(a.at), a.n, static_cast<const float*>(b.at), b.n);
+    };
+    for (const Span* o = outs.begin(); o != outs.end(); ++o) {
+        bool clash = false;
+        for (const Span* q = o + 1; q != outs.end(); ++q) clash = clash || share(*o, *q);
+        for (const Span* i = ins.begin(); i != ins.end(); ++i) {
+            const bool in_place = gradient && o == outs.begin() && i == ins.begin() && o->at == i->at;
+            clash = clash || (!in_place && share(*o, *i));
+        }
+        if (clash) return fail(KAI_E_INVALID_ARG, "%s: two buffers overlap", name);
+    }
+    return KAI_OK;
+}
+
 int kai_softmax_top_distill(int device, float* py, float* ps, const float* px, const int* pidx, const float* pt, int64_t nrow,
                             int64_t ncol, int64_t ntop, const float* temp, void* stream) {
     KAI_TRY(no_host_path(device));
     KAI_TRY(distill_args("softmax_top_distill", nrow, ncol, ntop));
     if (nrow > 0 && (!py || !ps || !px || (ntop > 0 && (!pidx || !pt))))
         return fail(KAI_E_INVALID_ARG, "softmax_top_distill: null pointer");
+    const int64_t nt = nrow * ntop;
+    KAI_TRY(loss_buffers("softmax_top_distill", {{py, nrow}, {ps, 3 * nrow}}, {{px, nrow * ncol}, {pidx, nt}, {pt, nt}}, false));
     KAI_ENTER(device);
     if (nrow == 0) return KAI_OK;
     return loss_distill(st, py, ps, px, pidx, pt, nrow, ncol, ntop, temp, s);
@@ -1596,8 +1621,9 @@ int kai_softmax_top_distill_backward_x(int device, float* pgx, const float* pgy,
     KAI_TRY(distill_args("softmax_top_distill_backward_x", nrow, ncol, ntop));
     if (nrow > 0 && (!pgx || !px || !ps || (ntop > 0 && (!pidx || !pt))))
         return fail(KAI_E_INVALID_ARG, "softmax_top_distill_backward_x: null pointer");
-    if (partly_overlap(pgx, nrow * ncol, px, nrow * ncol))
-        return fail(KAI_E_INVALID_ARG, "softmax_top_distill_backward_x: pgx and px overlap without being one buffer");
+    const int64_t nt = nrow * ntop;
+    KAI_TRY(loss_buffers("softmax_top_distill_backward_x", {{pgx, nrow * ncol}},
+                         {{px, nrow * ncol}, {pgy, nrow}, {ps, 3 * nrow}, {pidx, nt}, {pt, nt}}, true));
     KAI_ENTER(device);
     if (nrow == 0) return KAI_OK;
     return loss_distill_backward(st, pgx, pgy, px, ps, pidx, pt, nrow, ncol, ntop, temp, s);
@@ -1610,8 +1636,9 @@ int kai_softmax_top_distill_step(int device, float* py, float* pgx, const float*
     KAI_TRY(distill_args("softmax_top_distill_step", nrow, ncol, ntop));
     if (nrow > 0 && (!py || !pgx || !px || (ntop > 0 && (!pidx || !pt))))
         return fail(KAI_E_INVALID_ARG, "softmax_top_distill_step: null pointer");
-    if (partly_overlap(pgx, nrow * ncol, px, nrow * ncol))
-        return fail(KAI_E_INVALID_ARG, "softmax_top_distill_step: pgx and px overlap without being one buffer");
+    const int64_t nt = nrow * ntop;
+    KAI_TRY(loss_buffers("softmax_top_distill_step", {{pgx, nrow * ncol}, {py, nrow}},
+                         {{px, nrow * ncol}, {pgy, nrow}, {pidx, nt}, {pt, nt}}, true));
     KAI_ENTER(device);
     if (nrow == 0) return KAI_OK;
     return loss_distill_step(st, py, pgx, pgy, px, pidx, pt, nrow, ncol, ntop, temp, s);
@@ -1625,6 +1652,8 @@ int kai_softmax_policy_loss(int device, float* py, float* plogp, float* ps, cons
     KAI_TRY(row_loss_args("softmax_policy_loss", nrow, ncol));
     if (nrow > 0 && (!py || !ps || !px || !pz || !padv))
         return fail(KAI_E_INVALID_ARG, "softmax_policy_loss: null pointer");
+    KAI_TRY(loss_buffers("softmax_policy_loss", {{py, nrow}, {plogp, nrow}, {ps, 3 * nrow}},
+                         {{px, nrow * ncol}, {pz, nrow}, {pold, nrow}, {pref, nrow}, {padv, nrow}}, false));
     KAI_ENTER(device);
     if (nrow == 0) return KAI_OK;
     return loss_policy(st, py, plogp, ps, px, pz, pold, pref, padv, nrow, ncol, clip_low, clip_high, kl_coef, temp, s);
@@ -1636,8 +1665,8 @@ int kai_softmax_policy_loss_backward_x(int device, float* pgx, const float* pgy,
     KAI_TRY(row_loss_args("softmax_policy_loss_backward_x", nrow, ncol));
     if (nrow > 0 && (!pgx || !px || !ps || !pz))
         return fail(KAI_E_INVALID_ARG, "softmax_policy_loss_backward_x: null pointer");
-    if (partly_overlap(pgx, nrow * ncol, px, nrow * ncol))
-        return fail(KAI_E_INVALID_ARG, "softmax_policy_loss_backward_x: pgx and px overlap without being one buffer");
+    KAI_TRY(loss_buffers("softmax_policy_loss_backward_x", {{pgx, nrow * ncol}},
+                         {{px, nrow * ncol}, {pgy, nrow}, {ps, 3 * nrow}, {pz, nrow}}, true));
     KAI_ENTER(device);
     if (nrow == 0) return KAI_OK;
     return loss_policy_backward(st, pgx, pgy, px, ps, pz, nrow, ncol, temp, s);
@@ -1651,8 +1680,8 @@ int kai_softmax_policy_loss_step(int device, float* py, float* plogp, float* pgx
     KAI_TRY(row_loss_args("softmax_policy_loss_step", nrow, ncol));
     if (nrow > 0 && (!py || !pgx || !px || !pz || !padv))
         return fail(KAI_E_INVALID_ARG, "softmax_policy_loss_step: null pointer");
-    if (partly_overlap(pgx, nrow * ncol, px, nrow * ncol))
-        return fail(KAI_E_INVALID_ARG, "softmax_policy_loss_step: pgx and px overlap without being one buffer");
+    KAI_TRY(loss_buffers("softmax_policy_loss_step", {{pgx, nrow * ncol}, {py, nrow}, {plogp, nrow}},
+                         {{px, nrow * ncol}, {pgy, nrow}, {pz, nrow}, {pold, nrow}, {pref, nrow}, {padv, nrow}}, true));
     KAI_ENTER(device);
     if (nrow == 0) return KAI_OK;
     return loss_policy_step(st, py, plogp, pgx, pgy, px, pz, pold, pref, padv, nrow, ncol, clip_low, clip_high, kl_coef,

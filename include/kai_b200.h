@@ -482,8 +482,8 @@ KAI_API int kai_gated_linear_backward(int device, float* pgx, float* pgwg, float
  * reads as 1.  Each comes as a forward call that saves three numbers per row in ps[nrow,3] (the exponent that the row's
  * exponentials are taken against, their sum, d loss / d log-probability), a backward call that reads them, and a _step call
  * that does both with one read of px, for callers that know the loss's gradient pgy[nrow] beforehand (NULL reads as 1
- * for every row).  pgx may
- * be px itself in the backward and _step calls; any other overlap is not allowed.  Rows without a label
+ * for every row).  pgx may be px itself in the backward and _step calls; no other output may overlap another of the call's
+ * buffers (KAI_E_INVALID_ARG).  Rows without a label
  * (pz[r] = -1, or no used entry that has a weight) are padding: loss and gradient 0, whatever the logits hold.  Labels are checked on
  * the device: any other label outside [0, ncol) makes the row's loss and gradient NaN and is reported by
  * kai_device_status (KAI_E_OUT_OF_RANGE).  A logit of -inf, or one so low that logit / temp * log2(e) leaves the range of

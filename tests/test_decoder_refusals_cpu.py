@@ -103,3 +103,32 @@ def test_rotary_rows_against_a_list_of_every_value():
 ])
 def test_more_bytes_than_addresses(name, changes):
     assert _call(name, changes) == LARGE
+
+
+# row losses: 4 rows of 100 columns (1600 bytes), 8 labels (128 bytes), per-row vectors of 16 bytes, statistics of 48
+@pytest.mark.parametrize("name,changes", [
+    ("kai_softmax_top_distill", {1: C + 1584}), ("kai_softmax_top_distill", {2: C}), ("kai_softmax_top_distill", {2: C - 44}),
+    ("kai_softmax_top_distill", {1: B + 32}), ("kai_softmax_top_distill", {1: D}), ("kai_softmax_top_distill", {2: E + 124}),
+    ("kai_softmax_top_distill_backward_x", {2: A + 16}), ("kai_softmax_top_distill_backward_x", {4: A + 1596}),
+    ("kai_softmax_top_distill_backward_x", {5: A}), ("kai_softmax_top_distill_backward_x", {1: F - 1596}),
+    ("kai_softmax_top_distill_step", {1: B}), ("kai_softmax_top_distill_step", {3: A}), ("kai_softmax_top_distill_step", {3: B + 800}),
+    ("kai_softmax_top_distill_step", {1: D + 4}), ("kai_softmax_top_distill_step", {2: E}),
+    ("kai_softmax_policy_loss", {1: D}), ("kai_softmax_policy_loss", {2: A}), ("kai_softmax_policy_loss", {3: A - 44}),
+    ("kai_softmax_policy_loss", {2: E}), ("kai_softmax_policy_loss", {1: H + 12}), ("kai_softmax_policy_loss", {3: G}),
+    ("kai_softmax_policy_loss_backward_x", {5: A + 4}), ("kai_softmax_policy_loss_backward_x", {2: A}),
+    ("kai_softmax_policy_loss_backward_x", {4: A + 1552}),
+    ("kai_softmax_policy_loss_step", {4: A}), ("kai_softmax_policy_loss_step", {2: A}), ("kai_softmax_policy_loss_step", {1: B + 1584}),
+    ("kai_softmax_policy_loss_step", {2: D}), ("kai_softmax_policy_loss_step", {9: B + 1596}), ("kai_softmax_policy_loss_step", {7: B}),
+    ("kai_softmax_policy_loss_step", {8: A}),
+])
+def test_row_loss_buffers_that_overlap(name, changes):
+    assert _call(name, changes) == BAD
+    assert b"overlap" in capi.load().kai_last_error_string()
+
+
+def test_row_loss_neighbours_are_no_overlap():
+    _on_the_device("kai_softmax_top_distill", {1: C + 1600, 2: C - 48})
+    _on_the_device("kai_softmax_top_distill_step", {4: B, 1: B + 1600, 3: B - 16})
+    _on_the_device("kai_softmax_policy_loss", {1: A, 2: A + 16, 3: A + 32, 4: A + 80})
+    _on_the_device("kai_softmax_policy_loss_step", {2: A + 16, 5: B, 9: B + 1600, 7: B + 1616, 8: B + 1616})
+    _on_the_device("kai_softmax_policy_loss_backward_x", {3: A, 2: A + 1600})
