@@ -26,20 +26,29 @@ def _ptr(x):
     raise ValueError("tensor arguments must be contiguous (the reference has no strides)")
 
 
-_type_names = {}     # torch.dtype -> its text, which torch puts together anew on every call
+def _taker(name):
+    """_ptr of an argument that has to be a tensor of this type (its text): another type would be misread, or read past its end,
+    not converted."""
+    known = None      # the type itself, once an argument has shown it (its text is put together anew on every call)
+
+    def take(x):
+        nonlocal known
+        if x is None or type(x) is int:
+            return x
+        try:
+            if x.dtype is known and x.is_contiguous():
+                return x.data_ptr()
+            if str(x.dtype) != name:
+                raise TypeError(f"a tensor of {name} is needed here, got {x.dtype}")
+            known = x.dtype
+        except AttributeError:
+            pass
+        return _ptr(x)
+
+    return take
 
 
-def _typed(x, name):
-    """_ptr of an argument that is not fp32 (`name`: the type's text): another type would be misread, not converted."""
-    if x is None or type(x) is int:
-        return x
-    kind = getattr(x, "dtype", None)
-    text = _type_names.get(kind)
-    if text is None and kind is not None:
-        text = _type_names[kind] = str(kind)
-    if text != name and kind is not None:
-        raise TypeError(f"a tensor of {name} is needed here, got {kind}")
-    return _ptr(x)
+_f32, _f64, _i32, _i64 = (_taker("torch." + t) for t in ("float32", "float64", "int32", "int64"))
 
 
 def _act(a) -> int:
@@ -276,75 +285,75 @@ def rotary(device, py, px, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot,
            ldx=None, stream=None):
     """Turns the pairs of every head by position * frequency; `layout` is "half" or "interleaved"."""
     nvec = nhead * npiece
-    capi.call("kai_rotary", device, _ptr(py), _ptr(px), _typed(pfreq, "torch.float64"), _typed(ppos, "torch.int64"), pos0, nbat, ntimes,
-              nhead, npiece, nrot, capi.ROTARY_LAYOUT[layout], _ptr(hScale), nvec if ldy is None else ldy,
+    capi.call("kai_rotary", device, _f32(py), _f32(px), _f64(pfreq), _i64(ppos), pos0, nbat, ntimes,
+              nhead, npiece, nrot, capi.ROTARY_LAYOUT[layout], _f32(hScale), nvec if ldy is None else ldy,
               nvec if ldx is None else ldx, _ptr(stream))
 
 
 def rotary_backward(device, pgx, pgy, pfreq, ppos, pos0, nbat, ntimes, nhead, npiece, nrot, layout="half", hScale=None,
                     ldgx=None, ldgy=None, stream=None):
     nvec = nhead * npiece
-    capi.call("kai_rotary_backward", device, _ptr(pgx), _ptr(pgy), _typed(pfreq, "torch.float64"), _typed(ppos, "torch.int64"), pos0,
-              nbat, ntimes, nhead, npiece, nrot, capi.ROTARY_LAYOUT[layout], _ptr(hScale), nvec if ldgx is None else ldgx,
+    capi.call("kai_rotary_backward", device, _f32(pgx), _f32(pgy), _f64(pfreq), _i64(ppos), pos0,
+              nbat, ntimes, nhead, npiece, nrot, capi.ROTARY_LAYOUT[layout], _f32(hScale), nvec if ldgx is None else ldgx,
               nvec if ldgy is None else ldgy, _ptr(stream))
 
 
 def rotary_frequencies(device, pfreq, nrot, base=10000.0, scaling="plain", factor=1.0, slow=1.0, fast=32.0, times=1,
                        stream=None):
     """nrot / 2 doubles, radians per position; `scaling` is "plain", "linear", "base" or "by_parts"."""
-    capi.call("kai_rotary_frequencies", device, _typed(pfreq, "torch.float64"), nrot, base, capi.ROTARY_SCALING[scaling], factor,
+    capi.call("kai_rotary_frequencies", device, _f64(pfreq), nrot, base, capi.ROTARY_SCALING[scaling], factor,
               slow, fast, times, _ptr(stream))
 
 
 def gated_linear_forward(device, ph, pg, pu, pwg, pwu, px, pbg, pbu, yvec, ndat, xvec, act="swish", leaky_alpha=None,
                          stream=None):
     """ph = act(px . pwg^T + pbg) * (px . pwu^T + pbu); pg / pu receive the two factors' sums for the backward call."""
-    capi.call("kai_gated_linear_forward", device, _ptr(ph), _ptr(pg), _ptr(pu), _ptr(pwg), _ptr(pwu), _ptr(px), _ptr(pbg),
-              _ptr(pbu), yvec, ndat, xvec, _act(act), _ptr(leaky_alpha), _ptr(stream))
+    capi.call("kai_gated_linear_forward", device, _f32(ph), _f32(pg), _f32(pu), _f32(pwg), _f32(pwu), _f32(px), _f32(pbg),
+              _f32(pbu), yvec, ndat, xvec, _act(act), _f32(leaky_alpha), _ptr(stream))
 
 
 def gated_linear_backward(device, pgx, pgwg, pgwu, pgg, pgu, pgh, pg, pu, pwg, pwu, px, yvec, ndat, xvec, act="swish",
                           leaky_alpha=None, acc_x=False, acc_w=False, stream=None):
-    capi.call("kai_gated_linear_backward", device, _ptr(pgx), _ptr(pgwg), _ptr(pgwu), _ptr(pgg), _ptr(pgu), _ptr(pgh),
-              _ptr(pg), _ptr(pu), _ptr(pwg), _ptr(pwu), _ptr(px), yvec, ndat, xvec, _act(act), _ptr(leaky_alpha),
+    capi.call("kai_gated_linear_backward", device, _f32(pgx), _f32(pgwg), _f32(pgwu), _f32(pgg), _f32(pgu), _f32(pgh),
+              _f32(pg), _f32(pu), _f32(pwg), _f32(pwu), _f32(px), yvec, ndat, xvec, _act(act), _f32(leaky_alpha),
               int(bool(acc_x)), int(bool(acc_w)), _ptr(stream))
 
 
 def softmax_top_distill(device, py, ps, px, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
     """py[r] = temp^2 * KL(teacher's listed entries || softmax(px[r] / temp)); ps[nrow, 3] is for the backward call."""
-    capi.call("kai_softmax_top_distill", device, _ptr(py), _ptr(ps), _ptr(px), _typed(pidx, "torch.int32"), _ptr(pt), nrow, ncol,
-              ntop, _ptr(hTemp), _ptr(stream))
+    capi.call("kai_softmax_top_distill", device, _f32(py), _f32(ps), _f32(px), _i32(pidx), _f32(pt), nrow, ncol,
+              ntop, _f32(hTemp), _ptr(stream))
 
 
 def softmax_top_distill_backward_x(device, pgx, pgy, px, ps, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
-    capi.call("kai_softmax_top_distill_backward_x", device, _ptr(pgx), _ptr(pgy), _ptr(px), _ptr(ps),
-              _typed(pidx, "torch.int32"), _ptr(pt), nrow, ncol, ntop, _ptr(hTemp), _ptr(stream))
+    capi.call("kai_softmax_top_distill_backward_x", device, _f32(pgx), _f32(pgy), _f32(px), _f32(ps),
+              _i32(pidx), _f32(pt), nrow, ncol, ntop, _f32(hTemp), _ptr(stream))
 
 
 def softmax_top_distill_step(device, py, pgx, pgy, px, pidx, pt, nrow, ncol, ntop, hTemp=None, stream=None):
     """Loss and gradient with one read of the logits, for a pgy that is known beforehand (None: 1 for every row)."""
-    capi.call("kai_softmax_top_distill_step", device, _ptr(py), _ptr(pgx), _ptr(pgy), _ptr(px), _typed(pidx, "torch.int32"),
-              _ptr(pt), nrow, ncol, ntop, _ptr(hTemp), _ptr(stream))
+    capi.call("kai_softmax_top_distill_step", device, _f32(py), _f32(pgx), _f32(pgy), _f32(px), _i32(pidx),
+              _f32(pt), nrow, ncol, ntop, _f32(hTemp), _ptr(stream))
 
 
 def softmax_policy_loss(device, py, plogp, ps, px, pz, pold, pref, padv, nrow, ncol, hClipLow=None, hClipHigh=None,
                         hKlCoef=None, hTemp=None, stream=None):
     """Clipped policy loss of the tokens pz, with a KL term against pref; plogp receives their log-probabilities."""
-    capi.call("kai_softmax_policy_loss", device, _ptr(py), _ptr(plogp), _ptr(ps), _ptr(px), _typed(pz, "torch.int32"), _ptr(pold),
-              _ptr(pref), _ptr(padv), nrow, ncol, _ptr(hClipLow), _ptr(hClipHigh), _ptr(hKlCoef), _ptr(hTemp), _ptr(stream))
+    capi.call("kai_softmax_policy_loss", device, _f32(py), _f32(plogp), _f32(ps), _f32(px), _i32(pz), _f32(pold),
+              _f32(pref), _f32(padv), nrow, ncol, _f32(hClipLow), _f32(hClipHigh), _f32(hKlCoef), _f32(hTemp), _ptr(stream))
 
 
 def softmax_policy_loss_backward_x(device, pgx, pgy, px, ps, pz, nrow, ncol, hTemp=None, stream=None):
-    capi.call("kai_softmax_policy_loss_backward_x", device, _ptr(pgx), _ptr(pgy), _ptr(px), _ptr(ps), _typed(pz, "torch.int32"),
-              nrow, ncol, _ptr(hTemp), _ptr(stream))
+    capi.call("kai_softmax_policy_loss_backward_x", device, _f32(pgx), _f32(pgy), _f32(px), _f32(ps), _i32(pz),
+              nrow, ncol, _f32(hTemp), _ptr(stream))
 
 
 def softmax_policy_loss_step(device, py, plogp, pgx, pgy, px, pz, pold, pref, padv, nrow, ncol, hClipLow=None,
                              hClipHigh=None, hKlCoef=None, hTemp=None, stream=None):
     """Loss and gradient with one read of the logits, for a pgy that is known beforehand (None: 1 for every row)."""
-    capi.call("kai_softmax_policy_loss_step", device, _ptr(py), _ptr(plogp), _ptr(pgx), _ptr(pgy), _ptr(px),
-              _typed(pz, "torch.int32"), _ptr(pold), _ptr(pref), _ptr(padv), nrow, ncol, _ptr(hClipLow), _ptr(hClipHigh),
-              _ptr(hKlCoef), _ptr(hTemp), _ptr(stream))
+    capi.call("kai_softmax_policy_loss_step", device, _f32(py), _f32(plogp), _f32(pgx), _f32(pgy), _f32(px),
+              _i32(pz), _f32(pold), _f32(pref), _f32(padv), nrow, ncol, _f32(hClipLow), _f32(hClipHigh),
+              _f32(hKlCoef), _f32(hTemp), _ptr(stream))
 
 
 class Replay:
