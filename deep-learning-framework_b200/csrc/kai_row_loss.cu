@@ -45,6 +45,7 @@
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "kai_common.cuh"
 #include "kai_tcgen05.cuh"
@@ -1052,14 +1053,15 @@ int row_parts(int64_t nrow, int64_t ncol, int64_t most, int sm_count) {
     return static_cast<int>(parts);
 }
 
-// Threads of a CTA: 64 for many short rows (a part of 2048 columns at most; those with more labels than row_short_kernel takes: 8192 x
-// 250, 200 labels, loss 29 us, with 128 threads 43), 256 for parts beyond kPartOne and where there are too
+// Threads of a CTA: 64 for many short rows (a part of 2048 columns at most; only rows with more labels than row_short_kernel takes get
+// here, so none of the policy loss: 8192 x 250, 200 labels, loss 29 us, with 128 threads 43), 256 for parts beyond kPartOne and where there are too
 // few parts to give every SM four, 128 otherwise.
 template <class L, int MODE>
 int launch_threads(DeviceState* st, const RowParams& p, const L& loss, cudaStream_t s) {
     const int64_t each = (p.ncol + p.parts - 1) / p.parts, ctas = p.nrow * p.parts;
     if (each > kPartOne || ctas < 4 * static_cast<int64_t>(st->sm_count)) return launch_stream<L, 256, MODE>(st, p, loss, s);
-    if (each <= 2048) return launch_stream<L, 64, MODE>(st, p, loss, s);
+    if constexpr (std::is_same_v<L, Distill>)
+        if (each <= 2048) return launch_stream<L, 64, MODE>(st, p, loss, s);
     return launch_stream<L, 128, MODE>(st, p, loss, s);
 }
 
