@@ -240,7 +240,7 @@ int ensure_aux(DeviceState* st, int64_t bytes) {
     if (bytes <= st->aux_bytes) return KAI_OK;
     if (capturing())
         return fail(KAI_E_ALLOC,
-                    "the scratch block of this convolution would have to grow to %lld bytes inside a stream capture; run "
+                    "the scratch block of this call would have to grow to %lld bytes inside a stream capture; run "
                     "the call list once outside the capture first", (long long)bytes);
     if (st->aux) {
         if (st->ws_recorded) st->ws_retired.push_back(st->aux);   // a recorded graph may still point into it

@@ -38,7 +38,10 @@ struct Options {
     std::atomic<int64_t> tc_bn{256};
     std::atomic<int64_t> tc_bk{16};
     std::atomic<int64_t> tc_min_flops{int64_t(1) << 29};  // below: SIMT kernel
-    std::atomic<int64_t> gated_tc_flops{1200000000};        // gated layer: flops of its forward products from which on the tensor-core GEMM takes them
+    // gated layer: flops of its forward products from which on the tensor-core GEMM takes them, in both directions.  391 x 512 -> 1365
+    // (1.09 GFLOP): 36 and 68 us below, 42 and 83 on that GEMM; 1024 x 512 -> 512 (1.07): 33 and 59, 32 and 62; few rows of large
+    // weights lose by it in the backward call (20 rows, 4096 -> 4096: 148 us below, 256 on the GEMM's planes).
+    std::atomic<int64_t> gated_tc_flops{1200000000};
     std::atomic<int64_t> gated_raw_rows{384};             // gated layer: most rows whose forward call works without operand planes
     std::atomic<int64_t> split_k{0};                      // 0 = automatic
     std::atomic<int64_t> path{KAI_PATH_AUTO};
@@ -88,7 +91,8 @@ struct DeviceState {
     // matrices of a convolution); the GEMM's own planes start behind them.
     int64_t    ws_front = 0;
     // Second scratch block: inputs that a convolution variant rewrites before it calls the plain convolution
-    // (channel-group sums, the upsampled image of a transposed convolution, permuted kernels), which uses `ws`.
+    // (channel-group sums, the upsampled image of a transposed convolution, permuted kernels), which uses `ws`; the row losses'
+    // statistics between their two kernels, where one call for loss and gradient is two.
     void*      aux = nullptr;
     int64_t    aux_bytes = 0;
     int*       flag_dev = nullptr;      // small device scratch (label range flag)

@@ -18,6 +18,10 @@
 // reduction and the weight gradients many with a short one, the CTAs of some clusters share a tile and those of
 // others take one each); each leaves its tile in its shared memory, and after a
 // cluster barrier every CTA finishes its share of the rows by adding the tiles in rank order (the same bits on every run).
+// Measured: 48 x 512 x 512 forward 10.5 us, 391 x 512 x 1365 forward 36, backward 68 us (the tensor-core GEMM: 42 and 83); 4096 x
+// 512 x 512 forward 84 us, 51 TFLOP/s.  The tensor pipe is busy 54 % (backward), the issue slots 49 %: per 96 MMAs a warp spends 64 operations
+// on loads, 192 on splits and 100 on copies and their bounds.  Part of that: operand blocks by ldmatrix and the bounds of a copy hoisted out of
+// its loop gained 12 %, four blocks per SM instead of three 17 %.
 #include <math.h>
 
 #include <initializer_list>
@@ -25,11 +29,6 @@
 #include "kai_act.cuh"
 #include "kai_common.cuh"
 
-//
-// Measured: 48 x 512 x 512 forward 10.5 us, 391 x 512 x 1365 forward 36, backward 69 us (the tensor-core GEMM: 39 and 86); 4096 x
-// 512 x 512 forward 84 us, 51 TFLOP/s.  The tensor pipe is busy 54 % (backward), the issue slots 49 %: per 96 MMAs a warp spends 64 operations
-// on loads, 192 on splits and 100 on copies and their bounds.  Tried: operand blocks by ldmatrix and the bounds of a copy hoisted, 12 %;
-// four blocks per SM instead of three, 17 %.
 namespace kai {
 namespace {
 

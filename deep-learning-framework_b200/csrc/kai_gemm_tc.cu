@@ -246,7 +246,7 @@ __device__ __forceinline__ int chunk_col(int half, int cc) {
     return (cc * 32 < Q) ? half * Q + cc * 32 : HALF + half * Q + (cc * 32 - Q);
 }
 
-// Outputs of 32 consecutive hidden units of one row of a gated tile.
+// Outputs of 4 consecutive hidden units of one row of a gated tile (the fix-up of range-split tiles).
 __device__ __forceinline__ void store_gated4(const TcParams& p, int64_t row, int64_t n0, const float* g, const float* u, bool vec_ok,
                                              float alpha) {
     const int64_t left = p.N - n0;
@@ -657,9 +657,9 @@ gemm_3xtf32_gated_kernel(const __grid_constant__ CUtensorMap map_a_hi, const __g
 // The same from the operands as they are: for a few rows of x the weights are read once, 4 bytes per value, instead of becoming
 // planes first.  48 rows of 4096 x 4096: 66 us with its fix-up, 141 us with planes (128 MiB of weights: 20.5 us at the copy rate).  The
 // tensor pipe is busy 44 % of the time, shared memory 36 %: a 16-wide block takes 2000 clocks, of which its MMAs need 768; the rest is the
-// hand-over between copy, split and MMA.  A ring of its own for the lo tiles (66 to 64 us), two groups of splitting warps in turns (68) and
-// loads batched ahead of the split (71, the sums then spill) were measured; rows of 256 and more: 129 against 203 us at 4096 x
-// 4096, level at 391 rows of 2048 x 2048, slower from 512 rows of 4096 x 4096 on (240 against 209).
+// hand-over between copy, split and MMA.  The ring of its own for the lo tiles gained 66 to 64 us; two groups of splitting warps in turns (68) and
+// loads batched ahead of the split (71, the sums then spill) are not in it.  With planes, at 4096 x 4096: 48 rows 140 us against 67, 128 rows
+// 150 against 83, 256 rows 203 against 134, 384 rows 231 against 254; level at 391 rows of 2048 x 2048.
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_3xtf32_gated_raw_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_g,
                              const __grid_constant__ CUtensorMap map_u, const TcParams p) {

@@ -25,23 +25,26 @@
 // registers stood in the way of the label warp's loads.  As it is: 431 to 445 us (4.8 TB/s), policy loss 4096 x 50257 324 us (5.1 TB/s),
 // loss alone 195 us (5.4 TB/s), two calls 550 us.  A part takes 17,000 to 24,000 clocks from load to store (3700 waiting
 // for its load, 3500 in the two passes, 3500 to 5000 at the cluster barrier, 2000 to 2700 for statistics and slope, 3000 for the
-// gradient, 2500 until the store has read its source), with 34 to 39 % of the issue slots used: it is bound by the latency of that
+// gradient, 2500 until the store has read its source), with 26 to 39 % of the issue slots used: it is bound by the latency of that
 // chain.  Measured without gain: parts of 4096 to 16384 columns, 64 to 256 threads, cluster sizes between the powers of two.
 // row_short_kernel takes rows of up to 4096 columns (kGrad with many rows: 2048) with up to 256 labels, a warp each: there the barriers and the label warp of
 // row_stream_kernel cost more than the row.  Loss and gradient of 8192 rows, the stream's time first: 97 columns, 64 labels 37 us and
 // 14.5; 1000 columns, 256 labels 155 and 40 (64 labels: 44 and 23); 2000 columns, 200 labels 123 and 50; policy loss, 8191 x 1000 29
 // and 17 (10 at the copy rate; bound by the chain of one row in the 24 warps per SM that its registers leave).
-// row_loss_wide_kernel takes the rows that the shared memory of a cluster cannot hold (more than 400000 columns), for kLoss;
+// row_loss_wide_kernel takes the rows that the shared memory of a cluster cannot hold (more than 445000 columns, 280000 with 2048 labels), for kLoss;
 // kStep is then kLoss and kGrad.
 //
 // Precision.  exp((x - m) / T) is formed as 2^(x c - k) with c = log2(e) / T and k = m c, each rounded once: one fused multiply-add,
 // rounded relative to the exponent itself; what k lost stands in every term and in the logarithm below alike, and rounding
-// c is a temperature off by 2^-24, the same for every term.  The largest term is 2^0 to within rounding: with k the integer above
+// c is a temperature off by 2^-24 at most, the same for every term: log q is off by as much of the difference between the label's argument and
+// the row's mean one (a label 20 below the maximum: 1.2e-6 at most; a label's logarithm with the exact factor over a sum with the rounded
+// one is further off in most rows).  The largest term is 2^0 to within rounding: with k the integer above
 // m c, which joins sums by exact powers of two, it is a power of a fraction, and the instruction's 2^-22 on a term that is nearly
 // the whole sum cost log-probabilities next to 0 three binary digits (a policy row of 1e-6 relative error, 2e-7 so).
 // Exponentials and their sums are fp32 (a few dozen values per thread, then joined in a fixed order); log q = ln 2 (x c - k) - log(sum) is formed in 64 bits per row, with
 // the logarithm of the sum split into exponent and mantissa: log(sum) rounded to fp32 would alone be off by up to
-// 5e-7, which the ratio of two probabilities and a clip bound next to it would see.
+// 5e-7, which the ratio of two probabilities and a clip bound next to it would see.  Sums measured 2e-8 to 8e-8 low on average (the
+// instruction), 7e-8 to 1.2e-7 off (root mean square, 1000 to 128256 columns); the ratio of a policy row 8e-8 to 2e-7.
 #include <math.h>
 
 #include <mutex>

@@ -424,7 +424,13 @@ KAI_API int kai_sum_backward(int device, float* pgx, const float* pgy, int64_t n
 /* ---- decoder training: rotary positions, gated linear layer, losses on logits ---------------
  * No counterpart in the reference: what a decoder needs next to matmul, the attention trio and
  * softmax_idx_crossentropy.  Same conventions as above (dense fp32 rows, HYPER pointers, `device`,
- * `stream`); all of them are asynchronous and may be recorded. */
+ * `stream`); all of them are asynchronous and may be recorded.
+ *
+ * Scratch: kai_gated_linear_forward and _backward may use the device's workspace (from "gated_tc_flops" on), the two
+ * _step calls its second scratch block (rows of more than 445000 columns, 280000 with KAI_TOP_MAX labels).  Calls that use either,
+ * these or others of the library, must not overlap on the GPU: on one device they belong on one stream, and
+ * recorded lists that hold them are not replayed side by side.  A recorded call cannot make its scratch grow (KAI_E_ALLOC):
+ * make it once outside.  kai_rotary*, the loss-only and _backward_x calls use none. */
 
 /* Rotary positions.  The first nrot (even) of a head's npiece values form nrot / 2 pairs (a_i, b_i), which are turned
  * by the angle pos * pfreq[i]:
