@@ -43,8 +43,9 @@
 // the whole sum cost log-probabilities next to 0 three binary digits (a policy row of 1e-6 relative error, 2e-7 so).
 // Exponentials and their sums are fp32 (a few dozen values per thread, then joined in a fixed order); log q = ln 2 (x c - k) - log(sum) is formed in 64 bits per row, with
 // the logarithm of the sum split into exponent and mantissa: log(sum) rounded to fp32 would alone be off by up to
-// 5e-7, which the ratio of two probabilities and a clip bound next to it would see.  Sums measured 2e-8 to 8e-8 low on average (the
-// instruction), 7e-8 to 1.2e-7 off (root mean square, 1000 to 128256 columns); the ratio of a policy row 8e-8 to 2e-7.
+// 5e-7, which the ratio of two probabilities and a clip bound next to it would see.  The instruction's results are 5e-8 low on average
+// wherever its argument lies, and are taken twice where warps' sums are joined: sums measured 2e-8 to 8e-8 low, 7e-8 to 1.2e-7 off (root mean
+// square, 1000 to 128256 columns); the ratio of a policy row 8e-8 to 2e-7.
 #include <math.h>
 
 #include <mutex>
